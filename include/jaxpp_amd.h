@@ -267,7 +267,9 @@ typedef enum {
   JPP_WS_MSE = 3,              /* jpp_mse_loss partial */
   JPP_WS_MOE_WORK = 4,         /* jpp_moe_args.work: d0 = tokens, d1 = n_experts */
   JPP_WS_MOE_ROUTER_WGRAD = 5, /* jpp_moe_router_wgrad partial: d0 = hidden, d1 = n_experts */
-  JPP_WS_SPLIT_WGRAD = 6       /* `parts` of jpp_sum_accum_f32: d0 = n_parts, d1 = rows, d2 = cols */
+  JPP_WS_SPLIT_WGRAD = 6,      /* `parts` of jpp_sum_accum_f32: d0 = n_parts, d1 = rows, d2 = cols */
+  JPP_WS_BLOCK_JOIN = 7,       /* jpp_join_args.workspace: d0 = cols, d1 = rows / gate_rows (1 without a gate) */
+  JPP_WS_DISTILL = 8           /* jpp_distill_args.workspace: d0 = rows */
 } jpp_workspace_op;
 size_t jpp_workspace_bytes(int op, int64_t d0, int64_t d1, int64_t d2);
 
@@ -429,6 +431,103 @@ int jpp_moe_combine_bwd(void* stream, const jpp_moe_args* args, const void* dxp,
 /* acc[hidden, n_experts] += x^T dlogits; partial: f32 [64 * hidden * n_experts] */
 int jpp_moe_router_wgrad(void* stream, const jpp_moe_args* args, const void* x,
                          const float* dlogits, float* acc, float* partial);
+
+/* ---- linear attention with a decay for each head ---------------------------------
+ * No counterpart in the reference, whose models attend with a softmax: the token mixer of a student whose cost is linear
+ * in the length.  Per sequence and query head (key / value head h / (n_heads / n_kv_heads)), lambda = exp(decay[h]):
+ *   S_t = lambda S_{t-1} + k_t^T v_t,    o_t = scale q_t S_t,    S_{-1} = state_in (zero without)
+ * Tensors as for jpp_attn_fwd: row b * seq + t, head h at columns h * head_dim; any seq >= 0, head_dim 64 or 128.
+ * Rows from lens[b] on (lens: device int32 [batch], held to 0 .. seq; NULL: seq everywhere) are not read; their
+ * results are zero and the state passes them by.  States are f32, S[d][e] of key feature d and value feature e,
+ * also where the tensors are bf16.  decay is a constant of the layer: log of the head's factor, <= 0 (-inf: no memory).
+ * Outputs overlap no input but state_out, which may be state_in.  Results do not depend on timing. */
+typedef struct {
+  const void* q; const void* k; const void* v;
+  void* o;                  /* fwd, step: out */
+  const void* d_o;          /* bwd */
+  void* dq; void* dk; void* dv;
+  const float* decay;       /* f32 [n_heads] */
+  const float* state_in;    /* f32 [batch, n_heads, head_dim, head_dim] or NULL */
+  float* state_out;         /* the same, or NULL (fwd); S behind the last row */
+  const float* d_state_out; /* bwd: cotangent of state_out, or NULL */
+  float* d_state_in;        /* bwd: cotangent of state_in, or NULL; overlaps neither of those */
+  const int32_t* lens;
+  void* workspace;          /* jpp_linattn_workspace_bytes; may be NULL where that is 0 */
+  int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+  int batch, seq, n_heads, n_kv_heads, head_dim;
+  float scale;
+  int dtype;                /* jpp_dtype of q, k, v, o and their cotangents */
+} jpp_linattn_args;
+
+/* Scratch of a forward (backward = 0) or backward with these sizes (nothing else is read); 0 also for sizes that the call
+ * would refuse. */
+size_t jpp_linattn_workspace_bytes(const jpp_linattn_args* args, int backward);
+int jpp_linattn_fwd(void* stream, const jpp_linattn_args* args);
+/* dq, dk (summed over the query heads that share it), dv and d_state_in; the forward's states are computed again. */
+int jpp_linattn_bwd(void* stream, const jpp_linattn_args* args);
+/* One token per sequence: q, k, v, o of `batch` rows, state_in to state_out (required).  seq, lens and workspace are
+ * not read. */
+int jpp_linattn_step(void* stream, const jpp_linattn_args* args);
+
+/* ---- joining a block to the residual stream --------------------------------------
+ * No counterpart in the reference.  One pass for what stands between two blocks: the norm of a block's output, its gate,
+ * the scaled residual, and the norm in front of the next block (all norms are RMSNorms):
+ *   n = b * rstd_post * gamma_post    (gamma_post NULL: n = b)        rstd(z) = 1 / sqrt(mean(z^2) + eps)
+ *   h = alpha * x + gate * n          (gate NULL: 1)
+ *   y = h * rstd_pre * gamma_pre      (gamma_pre NULL: no y)
+ * x, b, h, y and their cotangents [rows, cols]; the gate is [rows / gate_rows, cols]: row r takes gate row
+ * r / gate_rows (one vector: gate_rows = rows; one for each sequence: gate_rows = seq).  y is computed from h
+ * before h is rounded.  cols at most 8192 and a multiple of 8 (f32: 4). */
+typedef struct {
+  const void* x;            /* fwd */
+  const void* b;            /* fwd, bwd */
+  const void* gamma_post;   /* [cols] or NULL */
+  const void* gate;         /* [rows / gate_rows, cols] or NULL */
+  const void* gamma_pre;    /* [cols] or NULL */
+  void* h;                  /* fwd: out (may be x or b); bwd: in (read only with gamma_pre) */
+  void* y;                  /* fwd: out; with gamma_pre */
+  float* rstd_post;         /* f32 [rows]; with gamma_post.  fwd: out, bwd: in */
+  float* rstd_pre;          /* f32 [rows]; with gamma_pre */
+  /* bwd: dh, the cotangent of h from what else reads it (NULL: none), and dy (with gamma_pre) give
+   *   dH = dh + d norm_pre(dy);  dx = alpha dH;  db = d norm_post(gate dH)
+   * and the sums over rows dgamma_pre, dgamma_post [cols], dgate [rows / gate_rows, cols], f32, each added to what is there
+   * if `accumulate`, else written (any of them NULL: not wanted).  dx may be dh or dy; db may be b. */
+  const void* dh; const void* dy;
+  void* dx; void* db;
+  float* dgamma_post; float* dgate; float* dgamma_pre;
+  void* workspace;          /* bwd: jpp_workspace_bytes(JPP_WS_BLOCK_JOIN, cols, rows / gate_rows, 0) bytes */
+  int64_t rows, cols, gate_rows;
+  float alpha, eps;
+  int accumulate;
+  int dtype;                /* jpp_dtype of all but the f32 pointers */
+} jpp_join_args;
+int jpp_block_join_fwd(void* stream, const jpp_join_args* args);
+int jpp_block_join_bwd(void* stream, const jpp_join_args* args);
+
+/* ---- distillation from a teacher's top logits -----------------------------------
+ * No counterpart in the reference (whose examples end in jpp_mse_loss's loss).  The loss of a student's logits against the
+ * teacher's `k` largest ones, and its gradient.  Per row, T = temperature, over the listed ids only for p, over
+ * the vocabulary for q:
+ *   p = softmax(teacher / T),  q = softmax(logits / T),  row_loss = weight T^2 sum_k p_k (log p_k - log q_k)
+ *   loss[0] = scale sum_rows row_loss,      dlogits = scale weight T (q - p)
+ * An id outside [0, vocab) is padding, an id that is listed twice counts twice; k = 1 is the cross entropy of that id (at
+ * T = 1).  A row with weight 0, or whose listed teacher logits are all -inf or padding, has no loss and no gradient, whatever
+ * its logits hold.  A masked student logit (-inf) has q = 0. */
+typedef struct {
+  const void* logits;       /* [rows, vocab], leading dimension ld; 16-byte aligned, any ld >= vocab */
+  const int32_t* ids;       /* [rows, k] */
+  const float* teacher;     /* f32 [rows, k] */
+  const float* weight;      /* f32 [rows] or NULL (1) */
+  float* row_loss;          /* f32 [rows] */
+  float* loss;              /* f32 [1] or NULL */
+  void* dlogits;            /* [rows, vocab], leading dimension ldd, or NULL (loss only); may be logits (with ldd = ld) */
+  void* workspace;          /* jpp_workspace_bytes(JPP_WS_DISTILL, rows, 0, 0) bytes; NULL: a row is one workgroup's */
+  int64_t ld, ldd, rows, vocab;
+  int k;                    /* 1 .. 1024 */
+  float temperature, scale;
+  int dtype;                /* jpp_dtype of logits and dlogits */
+} jpp_distill_args;
+int jpp_distill_loss(void* stream, const jpp_distill_args* args);
 
 /* ---- stage executor: stands in for `task_impl` on one pipeline rank ----------
  * A stage object holds this rank's chunks (the stages the schedule places on

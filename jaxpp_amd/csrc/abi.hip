@@ -323,6 +323,8 @@ size_t jpp_workspace_bytes(int op, int64_t d0, int64_t d1, int64_t d2) {
     case JPP_WS_MOE_WORK: return (size_t)2 * ((d0 + 255) / 256) * d1 * 4;
     case JPP_WS_MOE_ROUTER_WGRAD: return (size_t)64 * d0 * d1 * 4;
     case JPP_WS_SPLIT_WGRAD: return (size_t)d0 * d1 * d2 * 4;
+    case JPP_WS_BLOCK_JOIN: return (size_t)2 * (d1 + 512) * d0 * 4;
+    case JPP_WS_DISTILL: return (size_t)(d0 < 256 ? d0 : 0) * 64 * 8;   // rows few enough to be split, 64 pieces
     default: return 0;
   }
 }

@@ -1,0 +1,451 @@
+// What stands between two blocks of a stage in one pass over the rows: the norm of a block's output, its gate, the
+// scaled residual, the next block's norm - and the gradients of all of it.
+//
+//   n = b r_b gamma_post,  h = alpha x + gate n,  y = h r_h gamma_pre,        r_z = 1 / sqrt(mean(z^2) + eps)
+//
+//   dH = dh + r_h (t - h^ mean(t h^)),         t = dy gamma_pre,  h^ = h r_h
+//   dx = alpha dH
+//   db = r_b (u - b^ mean(u b^)),              u = dH gate gamma_post,  b^ = b r_b
+//   dgamma_pre = sum_rows dy h^;   with E = sum_rows dH b^ per row of the gate:
+//   dgate = gamma_post E,   dgamma_post = sum over the gate's rows of gate E
+//
+// HBM-bound: forward reads two tensors and writes two, backward reads four and writes two.  A row lives in
+// the registers of one wave or of one workgroup between its reductions.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+constexpr int kMaxCols = 8192;
+constexpr int kJoinParts = 512;     // workgroups of a backward, each with a line of partial sums
+
+// 16 bytes of a row as floats and back
+template <class E> struct Unit;
+template <> struct Unit<bf16_t> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) { unpack8(v, f); }
+  static __device__ __forceinline__ uint4 put(const float (&f)[8]) { return pack8(f); }
+};
+template <> struct Unit<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const uint4& v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+
+// Sum over the TPR threads of a row.  `red`: LDS of this reduction alone (a later one takes another).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if constexpr (TPR == 256) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0] + red[1] + red[2] + red[3];
+  }
+  return v;
+}
+
+struct JoinParams {
+  const void *x, *b, *gamma_post, *gate, *gamma_pre, *dh, *dy;
+  void *h, *y, *dx, *db;
+  float *rstd_post, *rstd_pre, *sum_e, *sum_f;
+  long rows, gate_rows;
+  int cols, splits;
+  float alpha, eps;
+};
+
+template <class E, int TPR, int NCH>
+__global__ __launch_bounds__(256) void block_join_fwd_kernel(JoinParams p) {
+  constexpr int N = Unit<E>::N;
+  __shared__ float red[8];
+  const int t = threadIdx.x % TPR;
+  const long row = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (row >= p.rows) return;        // whole rows of threads; a workgroup of one row has none of these
+  const int units = p.cols / N;
+  const uint4* xr = (const uint4*)((const E*)p.x + row * p.cols);
+  const uint4* br = (const uint4*)((const E*)p.b + row * p.cols);
+  const uint4* gr = p.gate ? (const uint4*)((const E*)p.gate + row / p.gate_rows * p.cols) : nullptr;
+  uint4 vb[NCH], vx[NCH];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = t + TPR * i;
+    vb[i] = c < units ? br[c] : make_uint4(0, 0, 0, 0);
+    vx[i] = c < units ? xr[c] : make_uint4(0, 0, 0, 0);
+  }
+  float rb = 1.f;
+  if (p.gamma_post) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      float f[N];
+      Unit<E>::get(vb[i], f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += f[e] * f[e];
+    }
+    rb = 1.0f / sqrtf(row_sum<TPR>(s, red) / p.cols + p.eps);
+    if (t == 0) p.rstd_post[row] = rb;
+  }
+  float h[NCH][N], s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = t + TPR * i;
+    float f[N], w[N];
+    Unit<E>::get(vx[i], h[i]);
+    Unit<E>::get(vb[i], f);
+    if (c < units) {
+      if (p.gamma_post) {
+        Unit<E>::get(((const uint4*)p.gamma_post)[c], w);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= rb * w[e];
+      }
+      if (gr) {
+        Unit<E>::get(gr[c], w);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] *= w[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      h[i][e] = p.alpha * h[i][e] + f[e];
+      s += h[i][e] * h[i][e];
+    }
+    if (c < units) ((uint4*)((E*)p.h + row * p.cols))[c] = Unit<E>::put(h[i]);
+  }
+  if (!p.gamma_pre) return;
+  const float rh = 1.0f / sqrtf(row_sum<TPR>(s, red + 4) / p.cols + p.eps);
+  if (t == 0) p.rstd_pre[row] = rh;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = t + TPR * i;
+    if (c < units) {
+      float w[N];
+      Unit<E>::get(((const uint4*)p.gamma_pre)[c], w);
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e] *= h[i][e] * rh;
+      ((uint4*)((E*)p.y + row * p.cols))[c] = Unit<E>::put(w);
+    }
+  }
+}
+
+// Workgroup `part` of a gate row's `splits`: its share of that row's rows, and one line of the sums E and F over them.
+template <class E, int TPR, int NCH>
+__global__ __launch_bounds__(256) void block_join_bwd_kernel(JoinParams p) {
+  constexpr int N = Unit<E>::N, LANES = 256 / TPR;
+  extern __shared__ float lds[];      // 16 floats of reductions (TPR = 256), or 2 x LANES x cols sums (TPR = 64)
+  const int t = threadIdx.x % TPR, lane = threadIdx.x / TPR;
+  const int units = p.cols / N;
+  const long group = blockIdx.x / p.splits, part = blockIdx.x % p.splits;
+  const long per = (p.gate_rows + p.splits - 1) / p.splits;
+  const long first = group * p.gate_rows + part * per;
+  const long last = min(min(first + per, (group + 1) * p.gate_rows), p.rows);
+  const uint4* gr = p.gate ? (const uint4*)((const E*)p.gate + group * p.cols) : nullptr;
+  float se[NCH][N], sf[NCH][N];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i)
+#pragma unroll
+    for (int e = 0; e < N; ++e) se[i][e] = sf[i][e] = 0.f;
+  int turn = 0;
+  for (long row = first + lane; row < last; row += LANES, turn ^= 8) {
+    const long at = row * p.cols;
+    float total[NCH][N];
+    const float rh = p.gamma_pre ? p.rstd_pre[row] : 0.f;
+    const float rb = p.gamma_post ? p.rstd_post[row] : 1.f;
+    uint4 vb[NCH], vh[NCH], vy[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int c = t + TPR * i;
+      const bool in = c < units;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      vb[i] = in ? ((const uint4*)((const E*)p.b + at))[c] : zero;
+      vh[i] = in && p.gamma_pre ? ((const uint4*)((const E*)p.h + at))[c] : zero;
+      vy[i] = in && p.gamma_pre ? ((const uint4*)((const E*)p.dy + at))[c] : zero;
+      Unit<E>::get(in && p.dh ? ((const uint4*)((const E*)p.dh + at))[c] : zero, total[i]);
+    }
+    if (p.gamma_pre) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int c = t + TPR * i;
+        if (c < units) {
+          float w[N], h[N], y[N];
+          Unit<E>::get(((const uint4*)p.gamma_pre)[c], w);
+          Unit<E>::get(vh[i], h);
+          Unit<E>::get(vy[i], y);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            s += y[e] * w[e] * (h[e] * rh);
+            sf[i][e] += y[e] * (h[e] * rh);
+          }
+        }
+      }
+      s = row_sum<TPR>(s, lds + turn) / p.cols;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int c = t + TPR * i;
+        if (c < units) {
+          float w[N], h[N], y[N];
+          Unit<E>::get(((const uint4*)p.gamma_pre)[c], w);
+          Unit<E>::get(vh[i], h);
+          Unit<E>::get(vy[i], y);
+#pragma unroll
+          for (int e = 0; e < N; ++e) total[i][e] += rh * (y[e] * w[e] - h[e] * rh * s);
+        }
+      }
+    }
+    float u[NCH][N], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int c = t + TPR * i;
+      float b[N], w[N];
+      Unit<E>::get(vb[i], b);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        se[i][e] += total[i][e] * (b[e] * rb);
+        u[i][e] = total[i][e];
+      }
+      if (c < units) {
+        if (gr) {
+          Unit<E>::get(gr[c], w);
+#pragma unroll
+          for (int e = 0; e < N; ++e) u[i][e] *= w[e];
+        }
+        if (p.gamma_post) {
+          Unit<E>::get(((const uint4*)p.gamma_post)[c], w);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            u[i][e] *= w[e];
+            s += u[i][e] * (b[e] * rb);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) total[i][e] *= p.alpha;
+      }
+    }
+    if (p.gamma_post) s = row_sum<TPR>(s, lds + turn + 4) / p.cols;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int c = t + TPR * i;
+      if (c < units) {
+        float b[N];
+        Unit<E>::get(vb[i], b);
+        if (p.gamma_post)
+#pragma unroll
+          for (int e = 0; e < N; ++e) u[i][e] = rb * (u[i][e] - b[e] * rb * s);
+        ((uint4*)((E*)p.dx + at))[c] = Unit<E>::put(total[i]);
+        ((uint4*)((E*)p.db + at))[c] = Unit<E>::put(u[i]);
+      }
+    }
+  }
+  if (!p.sum_e) return;
+  const long line = (long)blockIdx.x * p.cols;
+  if constexpr (LANES == 1) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int c = t + TPR * i;
+      if (c < units)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          p.sum_e[line + c * N + e] = se[i][e];
+          p.sum_f[line + c * N + e] = sf[i][e];
+        }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int c = t + TPR * i;
+      if (c < units)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          lds[lane * p.cols + c * N + e] = se[i][e];
+          lds[(LANES + lane) * p.cols + c * N + e] = sf[i][e];
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.cols; c += 256) {
+      float a = 0.f, f = 0.f;
+#pragma unroll
+      for (int l = 0; l < LANES; ++l) {
+        a += lds[l * p.cols + c];
+        f += lds[(LANES + l) * p.cols + c];
+      }
+      p.sum_e[line + c] = a;
+      p.sum_f[line + c] = f;
+    }
+  }
+}
+
+// The lines' sums, in their order: 32 columns by 32 shares of the lines.  blockIdx.y = 0: dgamma_pre and
+// dgamma_post; beyond: dgate.
+template <class E>
+__global__ __launch_bounds__(1024) void block_join_sums_kernel(const float* sum_e, const float* sum_f, const E* gamma_post,
+                                                               const E* gate, float* dgamma_pre, float* dgamma_post,
+                                                               float* dgate, int cols, long groups, int splits,
+                                                               int accumulate) {
+  __shared__ float red[2][32][33];
+  const int c = threadIdx.x & 31, l = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
+  const bool in = col < cols;
+  auto value = [](const E* p) {
+    if constexpr (sizeof(E) == 2) return bf16_to_f32(*p);
+    else return *p;
+  };
+  auto leave = [&](float* to, float v) { *to = accumulate ? *to + v : v; };
+  auto fold = [&](int k) {          // sum over the shares, in order
+    float v = 0.f;
+    for (int i = 0; i < 32; ++i) v += red[k][i][c];
+    return v;
+  };
+  if (blockIdx.y == 0) {
+    float a = 0.f, f = 0.f;
+    if (in)
+      for (long line = l; line < groups * splits; line += 32) {
+        const float e = sum_e[line * cols + col];
+        a += gate ? e * value(gate + line / splits * cols + col) : e;
+        f += sum_f[line * cols + col];
+      }
+    red[0][l][c] = a;
+    red[1][l][c] = f;
+    __syncthreads();
+    if (in && l == 0 && dgamma_post) leave(dgamma_post + col, fold(0));
+    if (in && l == 1 && dgamma_pre) leave(dgamma_pre + col, fold(1));
+    return;
+  }
+  for (long g = blockIdx.y - 1; g < groups; g += gridDim.y - 1) {
+    float a = 0.f;
+    if (in)
+      for (int s = l; s < splits; s += 32) a += sum_e[(g * splits + s) * cols + col];
+    __syncthreads();
+    red[0][l][c] = a;
+    __syncthreads();
+    if (in && l == 0) leave(dgate + g * cols + col, fold(0) * (gamma_post ? value(gamma_post + col) : 1.f));
+  }
+}
+
+int check(const jpp_join_args* a, const char* who, bool backward) {
+  JPP_REQUIRE(a, "%s: null operand", who);
+  JPP_REQUIRE(a->dtype == JPP_DTYPE_BF16 || a->dtype == JPP_DTYPE_F32, "%s: dtype %d", who, a->dtype);
+  const int unit = a->dtype == JPP_DTYPE_F32 ? 4 : 8;
+  JPP_REQUIRE(a->rows >= 0 && a->cols > 0 && a->cols <= kMaxCols && a->cols % unit == 0,
+              "%s: %lld rows of %lld: cols must be a multiple of %d and at most %d", who, (long long)a->rows, (long long)a->cols,
+              unit, kMaxCols);
+  JPP_REQUIRE(a->rows < (int64_t)1 << 23, "%s: %lld rows are too many", who, (long long)a->rows);
+  if (a->rows == 0) return JPP_OK;
+  JPP_REQUIRE(a->b, "%s: null operand", who);
+  JPP_REQUIRE(!a->gate || (a->gate_rows > 0 && a->rows % a->gate_rows == 0), "%s: %lld rows in gate rows of %lld", who,
+              (long long)a->rows, (long long)a->gate_rows);
+  JPP_REQUIRE(!a->gamma_post || a->rstd_post, "%s: gamma_post and rstd_post go together", who);
+  JPP_REQUIRE(!a->gamma_pre || a->rstd_pre, "%s: gamma_pre and rstd_pre go together", who);
+  JPP_REQUIRE(!backward || a->gamma_pre || a->dh, "%s: no cotangent", who);
+  const void* fwd[] = {a->x, a->b, a->gamma_post, a->gate, a->gamma_pre, a->h, a->gamma_pre ? a->y : nullptr};
+  const void* bwd[] = {a->b, a->gamma_post, a->gate, a->gamma_pre, a->gamma_pre ? a->h : nullptr, a->dh,
+                       a->gamma_pre ? a->dy : nullptr, a->dx, a->db, a->workspace};
+  uintptr_t bits = 0;
+  if (backward)
+    for (const void* q : bwd) bits |= (uintptr_t)q;
+  else
+    for (const void* q : fwd) bits |= (uintptr_t)q;
+  JPP_REQUIRE(bits % 16 == 0, "%s: operands must keep 16-byte alignment", who);
+  return JPP_OK;
+}
+
+JoinParams params_of(const jpp_join_args* a) {
+  JoinParams p = {};
+  p.x = a->x; p.b = a->b; p.gamma_post = a->gamma_post; p.gate = a->gate; p.gamma_pre = a->gamma_pre;
+  p.dh = a->dh; p.dy = a->dy; p.h = a->h; p.y = a->y; p.dx = a->dx; p.db = a->db;
+  p.rstd_post = a->rstd_post; p.rstd_pre = a->rstd_pre;
+  p.rows = a->rows;
+  p.gate_rows = a->gate ? a->gate_rows : a->rows;
+  p.cols = (int)a->cols;
+  p.alpha = a->alpha;
+  p.eps = a->eps;
+  return p;
+}
+
+// Threads of a row and units of each: a wave up to two units a lane, a workgroup beyond.
+#define JPP_JOIN_BY_COLS(LAUNCH, E_)                                         \
+  do {                                                                       \
+    const int units_ = p.cols / Unit<E_>::N;                                 \
+    if (units_ <= 64) LAUNCH(E_, 64, 1);                                     \
+    else if (units_ <= 128) LAUNCH(E_, 64, 2);                               \
+    else if (units_ <= 256) LAUNCH(E_, 256, 1);                              \
+    else if (units_ <= 512) LAUNCH(E_, 256, 2);                              \
+    else if (units_ <= 1024) LAUNCH(E_, 256, 4);                             \
+    else if constexpr (Unit<E_>::N == 4) LAUNCH(E_, 256, 8);                 \
+  } while (0)
+
+template <class E>
+int forward(hipStream_t st, const JoinParams& p) {
+#define JPP_JF(E_, T_, C_)                                                                                              \
+  hipLaunchKernelGGL((block_join_fwd_kernel<E_, T_, C_>), dim3((unsigned)((p.rows + 256 / T_ - 1) / (256 / T_))),       \
+                     dim3(256), 0, st, p)
+  JPP_JOIN_BY_COLS(JPP_JF, E);
+#undef JPP_JF
+  JPP_LAUNCH_CHECK();
+  return JPP_OK;
+}
+
+template <class E>
+int backward(hipStream_t st, JoinParams p, const jpp_join_args* a) {
+  const long groups = p.rows / p.gate_rows;
+  const bool sums = a->dgamma_post || a->dgate || a->dgamma_pre;
+  p.splits = (int)std::min<long>(groups >= kJoinParts ? 1 : (kJoinParts + groups - 1) / groups, p.gate_rows);
+  p.sum_e = sums ? (float*)a->workspace : nullptr;
+  p.sum_f = sums ? p.sum_e + groups * p.splits * p.cols : nullptr;
+#define JPP_JB(E_, T_, C_)                                                                                          \
+  hipLaunchKernelGGL((block_join_bwd_kernel<E_, T_, C_>), dim3((unsigned)(groups * p.splits)), dim3(256),           \
+                     T_ == 256 ? 64 : 2 * (256 / T_) * p.cols * 4, st, p)
+  JPP_JOIN_BY_COLS(JPP_JB, E);
+#undef JPP_JB
+  JPP_LAUNCH_CHECK();
+  if (!sums) return JPP_OK;
+  const dim3 grid((p.cols + 31) / 32, 1 + (unsigned)(a->dgate ? std::min<long>(groups, 4096) : 0));
+  hipLaunchKernelGGL((block_join_sums_kernel<E>), grid, dim3(1024), 0, st, p.sum_e, p.sum_f, (const E*)p.gamma_post,
+                     (const E*)p.gate, a->dgamma_pre, a->dgamma_post, a->dgate, p.cols, groups, p.splits, a->accumulate);
+  JPP_LAUNCH_CHECK();
+  return JPP_OK;
+}
+
+}  // namespace
+
+extern "C" int jpp_block_join_fwd(void* stream, const jpp_join_args* a) {
+  const char* who = "block_join_fwd";
+  if (int rc = check(a, who, false)) return rc;
+  if (a->rows == 0) return JPP_OK;
+  JPP_REQUIRE(a->x && a->h && (!a->gamma_pre || a->y), "%s: null operand", who);
+  JPP_REQUIRE(!a->y || (a->y != a->h && a->y != a->x && a->y != a->b), "%s: y overlaps another tensor", who);
+  hipStream_t st = (hipStream_t)stream;
+  const JoinParams p = params_of(a);
+  const double n = (double)a->rows * a->cols, es = a->dtype == JPP_DTYPE_F32 ? 4 : 2;
+  ProbeScope probe(st, "block_join_fwd", 0, es * n * (a->gamma_pre ? 4 : 3));
+  return a->dtype == JPP_DTYPE_F32 ? forward<float>(st, p) : forward<bf16_t>(st, p);
+}
+
+extern "C" int jpp_block_join_bwd(void* stream, const jpp_join_args* a) {
+  const char* who = "block_join_bwd";
+  if (int rc = check(a, who, true)) return rc;
+  if (a->rows == 0 && (a->accumulate || !(a->dgamma_post || a->dgate || a->dgamma_pre))) return JPP_OK;
+  if (a->rows == 0) {                 // sums over no rows
+    for (float* s : {a->dgamma_post, a->dgamma_pre})
+      if (s)
+        if (int rc = jpp_fill_u32(s, 0, (size_t)a->cols, stream)) return rc;
+    return JPP_OK;
+  }
+  JPP_REQUIRE(a->dx && a->db && (!a->gamma_pre || (a->h && a->dy)), "%s: null operand", who);
+  JPP_REQUIRE(a->gamma_post || !a->dgamma_post, "%s: dgamma_post without gamma_post", who);
+  JPP_REQUIRE(a->gamma_pre || !a->dgamma_pre, "%s: dgamma_pre without gamma_pre", who);
+  JPP_REQUIRE(a->gate || !a->dgate, "%s: dgate without gate", who);
+  JPP_REQUIRE(!(a->dgamma_post || a->dgate || a->dgamma_pre) || a->workspace, "%s: no workspace", who);
+  JPP_REQUIRE(a->dx != a->db && a->dx != a->b && a->dx != a->h && a->db != a->h && a->db != a->dh && a->db != a->dy,
+              "%s: dx and db overlap other tensors", who);
+  hipStream_t st = (hipStream_t)stream;
+  const JoinParams p = params_of(a);
+  const double n = (double)a->rows * a->cols, es = a->dtype == JPP_DTYPE_F32 ? 4 : 2;
+  ProbeScope probe(st, "block_join_bwd", 0, es * n * (3 + (a->gamma_pre ? 2 : 0) + (a->dh ? 1 : 0)));
+  return a->dtype == JPP_DTYPE_F32 ? backward<float>(st, p, a) : backward<bf16_t>(st, p, a);
+}

@@ -1,0 +1,939 @@
+// Linear attention with a decay for each head: forward, backward and one token per sequence.
+//
+//   S_t = lambda S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t              (S: D x D, f32)
+//
+// Every tensor of the forward and of the backward is one and the same sum over pairs of rows,
+//
+//   out_i = sum over j <= i of lambda^(i-j) (x_i . y_j) z_j  +  lambda^(i+1) x_i S           forward in time
+//   out_i = sum over j >= i of lambda^(j-i) (x_i . y_j) z_j  +  lambda^(n-1-i) x_i U         backward in time
+//
+// (n rows, S / U the state that enters at the end the walk starts from; the state that leaves is
+// lambda^n S + sum_j u_j y_j^T z_j with u_j = lambda^(n-1-j), backward in time lambda^(j+1)):
+//
+//   o   x, y, z = q, k, v                      dk  x, y, z = v, dO, q   backward, state U^T
+//   dq  x, y, z = dO, v, k   state S^T         dv  x, y, z = k, q, dO   backward, state U
+//
+// so one pair of kernels, given the tensors by a "role", computes all of them.
+//
+// A workgroup walks a segment of a sequence in chunks of rows (bf16: 64): within a chunk the pairs
+// are products of tiles, between chunks the state is carried in f32 accumulators, each wave 32
+// of its columns.  Where batch x heads give too few workgroups, a sequence is cut into segments:
+// a first launch sums every segment's y^T z, a second carries them over the segments (small), and the
+// walk starts each segment from its state.
+#include <math.h>
+
+#include <algorithm>
+
+#include "attention_common.h"
+
+using jpp_attn::acc_to_frag;
+using jpp_attn::pack2;
+using jpp_attn::slabs_frag;
+
+namespace {
+
+constexpr int kChunk = 64;       // rows of a chunk, bf16
+constexpr int kChunkF32 = 32;    // and f32
+constexpr int kMaxRoles = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Role {
+  const void* x; const void* y; const void* z;
+  void* out;                     // rows of ldo elements; element type of x, or f32
+  long ldx, ldy, ldz, ldo;
+  int gx, gy, gz, go;            // query heads per head of each tensor
+  int reverse;                   // walk from the last row to the first
+  int init_transposed;           // `init` holds the state's transpose
+  int out_f32;
+  float a_pair, a_state, a_update;  // factors of the pair sum, of the state's part and of y^T z in the state
+  const float* init;             // [batch, heads, D, D] or null (zero)
+  float* final_state;            // [batch, heads, D, D] or null
+  float* parts;                  // [batch, heads, n_seg, D, D]: sums of the segments, then their states
+};
+
+struct Params {
+  Role role[kMaxRoles];
+  int n_roles;
+  const float* decay;
+  const int32_t* lens;
+  int batch, seq, heads, n_seg, seg_rows;
+};
+
+struct Place {
+  int role, seg, h, b;
+  int s0, s1;       // the segment's rows
+  int live;         // of them within the sequence
+  float g2;         // log2 of the head's decay
+};
+
+// An exponent of this size takes the neighbouring row's part to zero; a head whose decay is exactly
+// zero (log -inf) is held here so that 0 * -inf does not arise.
+constexpr float kLeastDecay = -100.f;
+
+__device__ __forceinline__ float log2_decay(const float* decay, int h) {
+  const float g = decay[h];
+  return (g < kLeastDecay ? kLeastDecay : g) * kLog2e;
+}
+__device__ __forceinline__ int rows_of(const Params& p, int b) {
+  return p.lens ? min(max(p.lens[b], 0), p.seq) : p.seq;
+}
+
+// Workgroups of one (segment, batch) follow each other over the heads, and the roles over those: what
+// they share is read at about the same time.
+__device__ __forceinline__ Place place(const Params& p) {
+  Place w;
+  unsigned i = blockIdx.x;
+  w.role = i % p.n_roles;
+  i /= p.n_roles;
+  w.h = i % p.heads;
+  i /= p.heads;
+  w.seg = i % p.n_seg;
+  w.b = i / p.n_seg;
+  w.s0 = w.seg * p.seg_rows;
+  w.s1 = min(w.s0 + p.seg_rows, p.seq);
+  w.live = min(max(rows_of(p, w.b) - w.s0, 0), w.s1 - w.s0);
+  w.g2 = log2_decay(p.decay, w.h);
+  return w;
+}
+
+__device__ __forceinline__ float decay_pow(float g2, int n) { return exp2f(g2 * (float)n); }
+
+// 8 floats -> the bf16 operand nearest to them, and what that leaves
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ bf16x8 split(f32x8& v) {
+  const bf16x8 hi = __builtin_convertvector(v, bf16x8);
+  v -= __builtin_convertvector(hi, f32x8);
+  return hi;
+}
+__device__ __forceinline__ f32x8 acc8(const f32x16& a, int base) {
+  return f32x8{a[base], a[base + 1], a[base + 2], a[base + 3], a[base + 4], a[base + 5], a[base + 6], a[base + 7]};
+}
+
+// ---------------------------------------------------------------------------
+// bf16 tiles: [64][D] in LDS as D / 64 swizzled slabs, staged through registers (rows behind
+// the sequence's end are not read and count as zero)
+// ---------------------------------------------------------------------------
+template <int D>
+struct Tile {
+  static constexpr int THREADS = 2 * D;              // D / 32 waves
+  static constexpr int BYTES = kChunk * D * 2;
+  static constexpr int UNITS = D / 8;                // 16-byte units of a row
+  static constexpr int PER = kChunk * UNITS / THREADS;
+  static_assert(PER == 4, "four units per thread");
+
+  static __device__ __forceinline__ void load(uint4 (&r)[PER], const bf16_t* src, long ld, int live) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
+      r[i] = row < live ? *(const uint4*)(src + row * ld + c * 8) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  static __device__ __forceinline__ uint8_t* unit(uint8_t* tile, int i) {
+    const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
+    return tile + (c >> 3) * 8192 + slab_off(row, c & 7);
+  }
+  static __device__ __forceinline__ void put(uint8_t* tile, const uint4 (&r)[PER]) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) *(uint4*)unit(tile, i) = r[i];
+  }
+};
+
+// z of one chunk as MFMA operand (contraction over the rows, in the accumulators' order), times
+// the rows' weights, in three parts that together hold all 24 bits of the products: the state
+// is an f32 result, and its terms are as exact as f32 products.
+template <int D>
+__device__ __forceinline__ void update_state(f32x16 (&S)[D / 32], const uint8_t* ytile, const bf16x8 (&zf)[4],
+                                             float g2, float a_update, int rows, bool reverse, int lane) {
+  const float keep = decay_pow(g2, rows);
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) S[t] *= keep;
+#pragma unroll
+  for (int st = 0; st < 4; ++st) {
+    f32x8 z = __builtin_convertvector(zf[st], f32x8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = st * 16 + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3);
+      // (rows behind the end are zero, and their exponent is kept from going the other way)
+      z[e] *= a_update * decay_pow(g2, reverse ? j + 1 : max(rows - 1 - j, 0));
+    }
+    bf16x8 part[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) part[i] = split(z);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      const bf16x8 yf = slab_frag_tr(ytile, kChunk, t * 32, st, lane);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(yf, part[i], S[t], 0, 0, 0);
+    }
+  }
+}
+
+// State tiles: wave w holds columns 32 w .. + 31; a lane column lane & 31, rows 32 t + 8 (r / 4) + 4 (lane / 32) + r % 4.
+template <int D>
+__device__ __forceinline__ void load_state(f32x16 (&S)[D / 32], const float* src, bool transposed, int wave, int lane) {
+  const int col = wave * 32 + (lane & 31), hh = lane >> 5;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = t * 32 + q * 8 + hh * 4;
+      if (transposed) {
+        const float4 v = *(const float4*)(src + (long)col * D + row);
+        S[t][4 * q] = v.x; S[t][4 * q + 1] = v.y; S[t][4 * q + 2] = v.z; S[t][4 * q + 3] = v.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[t][4 * q + e] = src[(long)(row + e) * D + col];
+      }
+    }
+}
+template <int D>
+__device__ __forceinline__ void store_state(const f32x16 (&S)[D / 32], float* dst, int wave, int lane) {
+  const int col = wave * 32 + (lane & 31), hh = lane >> 5;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dst[(long)(t * 32 + (r >> 2) * 8 + hh * 4 + (r & 3)) * D + col] = S[t][r];
+}
+
+template <class T>
+__device__ __forceinline__ const T* rows_at(const void* base, long ld, int group, const Params& p, const Place& w, int dim) {
+  return (const T*)base + ((long)w.b * p.seq + w.s0) * ld + (long)(w.h / group) * dim;
+}
+
+// ---------------------------------------------------------------------------
+// sums of the segments: parts[seg] = what the segment adds to the state that leaves it
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(2 * D, 2) void linattn_sum_kernel(Params p) {
+  using T = Tile<D>;
+  constexpr int DT = D / 32;
+  __shared__ __align__(1024) uint8_t smem[2 * T::BYTES];
+  uint8_t* const ytile = smem;
+  uint8_t* const ztile = smem + T::BYTES;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place w = place(p);
+  const Role& ro = p.role[w.role];
+  // the last segment's sum enters the state that leaves the sequence and nothing else
+  if (!ro.final_state && w.seg == (ro.reverse ? 0 : p.n_seg - 1)) return;
+  const bf16_t* y = rows_at<bf16_t>(ro.y, ro.ldy, ro.gy, p, w, D);
+  const bf16_t* z = rows_at<bf16_t>(ro.z, ro.ldz, ro.gz, p, w, D);
+  f32x16 S[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) S[t] = 0.f;
+  const int n = (w.live + kChunk - 1) / kChunk;
+  uint4 ry[T::PER], rz[T::PER];
+  auto fetch = [&](int i) {
+    const int c = ro.reverse ? n - 1 - i : i;
+    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, w.live - c * kChunk);
+    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, w.live - c * kChunk);
+  };
+  if (n) fetch(0);
+  for (int i = 0; i < n; ++i) {
+    const int c = ro.reverse ? n - 1 - i : i;
+    T::put(ytile, ry);
+    T::put(ztile, rz);
+    __syncthreads();
+    if (i + 1 < n) fetch(i + 1);
+    bf16x8 zf[4];
+#pragma unroll
+    for (int st = 0; st < 4; ++st) zf[st] = slab_frag_tr(ztile, kChunk, wave * 32, st, lane);
+    update_state<D>(S, ytile, zf, w.g2, ro.a_update, min(kChunk, w.live - c * kChunk), ro.reverse, lane);
+    __syncthreads();
+  }
+  store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
+}
+
+// ---------------------------------------------------------------------------
+// carry: parts[seg] becomes the state that enters the segment; one thread per 4 elements of a state
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
+  constexpr int BLOCKS = D * D / 1024;     // of one state
+  unsigned i = blockIdx.x;
+  const int e = ((i % BLOCKS) * 256 + threadIdx.x) * 4;
+  i /= BLOCKS;
+  const Role& ro = p.role[i % p.n_roles];
+  const unsigned bh = i / p.n_roles;
+  const int h = bh % p.heads, b = bh / p.heads;
+  const float g2 = log2_decay(p.decay, h);
+  const int len = rows_of(p, b);
+  float4 s = make_float4(0, 0, 0, 0);
+  if (ro.init) {
+    const float* src = ro.init + (long)bh * D * D;
+    if (ro.init_transposed) {
+      const int row = e / D, col = e % D;
+      s = make_float4(src[(long)col * D + row], src[(long)(col + 1) * D + row], src[(long)(col + 2) * D + row],
+                      src[(long)(col + 3) * D + row]);
+    } else {
+      s = *(const float4*)(src + e);
+    }
+  }
+  float* parts = ro.parts + (long)bh * p.n_seg * D * D + e;
+  for (int k = 0; k < p.n_seg; ++k) {
+    const int seg = ro.reverse ? p.n_seg - 1 - k : k;
+    float4* at = (float4*)(parts + (long)seg * D * D);
+    const float4 add = k + 1 < p.n_seg || ro.final_state ? *at : make_float4(0, 0, 0, 0);
+    *at = s;
+    const float keep = decay_pow(g2, min(max(len - seg * p.seg_rows, 0), p.seg_rows));
+    s = make_float4(s.x * keep + add.x, s.y * keep + add.y, s.z * keep + add.z, s.w * keep + add.w);
+  }
+  if (ro.final_state) *(float4*)(ro.final_state + (long)bh * D * D + e) = s;
+}
+
+// ---------------------------------------------------------------------------
+// the walk, bf16.  Per chunk: P^T = Y X^T in quadrants of 32 x 32 (weighted, rounded to bf16 in two parts,
+// shared through LDS); O^T = S^T X^T from the state's accumulators as they are, times the rows' decay,
+// plus Z^T P^T; then the state's update.
+// The state and the pairs meet the matrix cores as two bf16 each (16 bits): one would add, to
+// the rounding of the result, as much again.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
+  using T = Tile<D>;
+  constexpr int DT = D / 32, NW = D / 32;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* const xtile = smem;                       // later the chunk's result
+  uint8_t* const ytile = smem + T::BYTES;
+  uint8_t* const ztile = smem + 2 * T::BYTES;
+  uint8_t* const ptile = smem + 3 * T::BYTES;        // two parts of 8 KB, rows i, j in the accumulators' order
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hh = lane >> 5, li = lane & 31;
+  const Place w = place(p);
+  const Role& ro = p.role[w.role];
+  const bool rev = ro.reverse;
+  const bf16_t* x = rows_at<bf16_t>(ro.x, ro.ldx, ro.gx, p, w, D);
+  const bf16_t* y = rows_at<bf16_t>(ro.y, ro.ldy, ro.gy, p, w, D);
+  const bf16_t* z = rows_at<bf16_t>(ro.z, ro.ldz, ro.gz, p, w, D);
+  const long bh = (long)w.b * p.heads + w.h;
+
+  f32x16 S[DT];
+  const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
+  if (from) {
+    load_state<D>(S, from, p.n_seg == 1 && ro.init_transposed, wave, lane);
+  } else {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) S[t] = 0.f;
+  }
+  bool have_state = from != nullptr;
+  const bool keep_last = p.n_seg == 1 && ro.final_state;
+
+  const int n = (w.live + kChunk - 1) / kChunk;
+  uint4 rx[T::PER], ry[T::PER], rz[T::PER];
+  auto fetch = [&](int i) {
+    const int c = rev ? n - 1 - i : i;
+    T::load(rx, x + (long)c * kChunk * ro.ldx, ro.ldx, w.live - c * kChunk);
+    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, w.live - c * kChunk);
+    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, w.live - c * kChunk);
+  };
+  if (n) fetch(0);
+  for (int i = 0; i < n; ++i) {
+    const int c = rev ? n - 1 - i : i;
+    const int rows = min(kChunk, w.live - c * kChunk);
+    T::put(xtile, rx);
+    T::put(ytile, ry);
+    T::put(ztile, rz);
+    __syncthreads();
+    if (i + 1 < n) fetch(i + 1);
+
+#pragma unroll
+    for (int q = wave; q < 4; q += NW) {
+      const int jt = q >> 1, it = q & 1;
+      if (rev ? jt < it : jt > it) continue;       // no pair of these rows counts
+      f32x16 s;
+      s = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(slabs_frag<D>(ytile, jt * 32, ks, lane),
+                                                    slabs_frag<D>(xtile, it * 32, ks, lane), s, 0, 0, 0);
+      const int row = it * 32 + li;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = jt * 32 + (r >> 2) * 8 + hh * 4 + (r & 3);
+        const int far = rev ? j - row : row - j;
+        s[r] = far >= 0 ? s[r] * (ro.a_pair * decay_pow(w.g2, max(far, 0))) : 0.f;
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        f32x8 v = acc8(s, s2 * 8);
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+          *(bf16x8*)(ptile + part * 8192 + slab_off(row, (jt * 2 + s2) * 2 + hh)) = split(v);
+      }
+    }
+
+    f32x16 o[2];
+    o[0] = 0.f;
+    o[1] = 0.f;
+    if (have_state) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          f32x8 v = acc8(S[t], s2 * 8);
+          const bf16x8 hi = split(v), lo = split(v);
+#pragma unroll
+          for (int it = 0; it < 2; ++it) {
+            // row it * 32 + li, elements 32 t + 16 s2 + 4 hh .. + 3 and the same 8 further on
+            const int row = it * 32 + li, u = (t & 1) * 4 + s2 * 2;
+            const uint8_t* slab = xtile + (t >> 1) * 8192 + hh * 8;
+            const uint2 a = *(const uint2*)(slab + slab_off(row, u));
+            const uint2 b = *(const uint2*)(slab + slab_off(row, u + 1));
+            const bf16x8 xf = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y));
+            o[it] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, xf, o[it], 0, 0, 0);
+            o[it] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, xf, o[it], 0, 0, 0);
+          }
+        }
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int row = it * 32 + li;
+        o[it] *= ro.a_state * decay_pow(w.g2, rev ? max(rows - 1 - row, 0) : row + 1);
+      }
+    }
+    bf16x8 zf[4];
+#pragma unroll
+    for (int st = 0; st < 4; ++st) zf[st] = slab_frag_tr(ztile, kChunk, wave * 32, st, lane);
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        if (rev ? (st >> 1) < it : (st >> 1) > it) continue;
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+          o[it] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(zf[st], slab_frag(ptile + part * 8192, it * 32, st, lane), o[it],
+                                                          0, 0, 0);
+      }
+    if (ro.out_f32) {
+      float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D + wave * 32;
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+        if (it * 32 + li < rows)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *(float4*)(out + (long)(it * 32 + li) * ro.ldo + q * 8 + hh * 4) =
+                make_float4(o[it][4 * q], o[it][4 * q + 1], o[it][4 * q + 2], o[it][4 * q + 3]);
+    } else {
+      // x is no longer needed: its place takes the result, which leaves by whole rows
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int u = wave * 4 + q;
+          *(uint2*)(xtile + (u >> 3) * 8192 + slab_off(it * 32 + li, u & 7) + hh * 8) =
+              make_uint2(pack2(o[it][4 * q], o[it][4 * q + 1]), pack2(o[it][4 * q + 2], o[it][4 * q + 3]));
+        }
+    }
+    if (i + 1 < n || keep_last) update_state<D>(S, ytile, zf, w.g2, ro.a_update, rows, rev, lane);
+    have_state = true;
+    __syncthreads();
+    if (!ro.out_f32) {
+      bf16_t* out = (bf16_t*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D;
+#pragma unroll
+      for (int k = 0; k < T::PER; ++k) {
+        const int u = k * T::THREADS + threadIdx.x, row = u / T::UNITS, col = u % T::UNITS;
+        // (the unit this thread overwrites with the next chunk's x)
+        if (row < rows) *(uint4*)(out + row * ro.ldo + col * 8) = *(const uint4*)T::unit(xtile, k);
+      }
+    }
+  }
+  if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
+  // rows behind the sequence's end
+  const int unit = ro.out_f32 ? 4 : 8, units = D / unit;
+  for (int k = threadIdx.x; k < (w.s1 - w.s0 - w.live) * units; k += T::THREADS) {
+    const long at = ((long)w.b * p.seq + w.s0 + w.live + k / units) * ro.ldo + (long)(w.h / ro.go) * D + (k % units) * unit;
+    *(uint4*)((uint8_t*)ro.out + at * (ro.out_f32 ? 4 : 2)) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the same on f32 tensors: f32 MFMA (32x32x2), chunks of 32 rows, rows padded in LDS
+// ---------------------------------------------------------------------------
+template <int D>
+struct TileF {
+  static constexpr int THREADS = 2 * D;
+  static constexpr int LD = D + 4;                   // floats of a row: 16 bytes of padding turn the banks
+  static constexpr int BYTES = kChunkF32 * LD * 4;
+  static constexpr int UNITS = D / 4;
+  static constexpr int PER = kChunkF32 * UNITS / THREADS;
+  static __device__ __forceinline__ void load(float4 (&r)[PER], const float* src, long ld, int live) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
+      r[i] = row < live ? *(const float4*)(src + row * ld + c * 4) : make_float4(0, 0, 0, 0);
+    }
+  }
+  static __device__ __forceinline__ void put(float* tile, const float4 (&r)[PER]) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
+      *(float4*)(tile + row * LD + c * 4) = r[i];
+    }
+  }
+};
+
+__device__ __forceinline__ float elem(const float4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; }
+
+// zf[r]: z of row 8 (r / 4) + 4 (lane / 32) + r % 4 at this lane's column
+template <int D>
+__device__ __forceinline__ void update_state_f32(f32x16 (&S)[D / 32], const float* ytile, const float (&zf)[16], float g2,
+                                                 float a_update, int rows, bool reverse, int lane) {
+  const float keep = decay_pow(g2, rows);
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) S[t] *= keep;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int j = (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
+    const float z = zf[r] * (a_update * decay_pow(g2, reverse ? j + 1 : max(rows - 1 - j, 0)));
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+      S[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(ytile[j * TileF<D>::LD + t * 32 + (lane & 31)], z, S[t], 0, 0, 0);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(2 * D, 2) void linattn_sum_f32_kernel(Params p) {
+  using T = TileF<D>;
+  constexpr int DT = D / 32;
+  __shared__ __align__(16) float smem[2 * kChunkF32 * T::LD];
+  float* const ytile = smem;
+  float* const ztile = smem + kChunkF32 * T::LD;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place w = place(p);
+  const Role& ro = p.role[w.role];
+  if (!ro.final_state && w.seg == (ro.reverse ? 0 : p.n_seg - 1)) return;
+  const float* y = rows_at<float>(ro.y, ro.ldy, ro.gy, p, w, D);
+  const float* z = rows_at<float>(ro.z, ro.ldz, ro.gz, p, w, D);
+  f32x16 S[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) S[t] = 0.f;
+  const int n = (w.live + kChunkF32 - 1) / kChunkF32;
+  float4 ry[T::PER], rz[T::PER];
+  auto fetch = [&](int i) {
+    const int c = ro.reverse ? n - 1 - i : i;
+    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, w.live - c * kChunkF32);
+    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, w.live - c * kChunkF32);
+  };
+  if (n) fetch(0);
+  for (int i = 0; i < n; ++i) {
+    const int c = ro.reverse ? n - 1 - i : i;
+    T::put(ytile, ry);
+    T::put(ztile, rz);
+    __syncthreads();
+    if (i + 1 < n) fetch(i + 1);
+    float zf[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      zf[r] = ztile[((r >> 2) * 8 + (lane >> 5) * 4 + (r & 3)) * T::LD + wave * 32 + (lane & 31)];
+    update_state_f32<D>(S, ytile, zf, w.g2, ro.a_update, min(kChunkF32, w.live - c * kChunkF32), ro.reverse, lane);
+    __syncthreads();
+  }
+  store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
+}
+
+template <int D>
+__global__ __launch_bounds__(2 * D, 2) void linattn_walk_f32_kernel(Params p) {
+  using T = TileF<D>;
+  constexpr int DT = D / 32;
+  __shared__ __align__(16) float smem[3 * kChunkF32 * T::LD];
+  float* const xtile = smem;
+  float* const ytile = smem + kChunkF32 * T::LD;
+  float* const ztile = smem + 2 * kChunkF32 * T::LD;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hh = lane >> 5, li = lane & 31;
+  const Place w = place(p);
+  const Role& ro = p.role[w.role];
+  const bool rev = ro.reverse;
+  const float* x = rows_at<float>(ro.x, ro.ldx, ro.gx, p, w, D);
+  const float* y = rows_at<float>(ro.y, ro.ldy, ro.gy, p, w, D);
+  const float* z = rows_at<float>(ro.z, ro.ldz, ro.gz, p, w, D);
+  const long bh = (long)w.b * p.heads + w.h;
+
+  f32x16 S[DT];
+  const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
+  if (from) {
+    load_state<D>(S, from, p.n_seg == 1 && ro.init_transposed, wave, lane);
+  } else {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) S[t] = 0.f;
+  }
+  bool have_state = from != nullptr;
+  const bool keep_last = p.n_seg == 1 && ro.final_state;
+  const int n = (w.live + kChunkF32 - 1) / kChunkF32;
+  float4 rx[T::PER], ry[T::PER], rz[T::PER];
+  auto fetch = [&](int i) {
+    const int c = rev ? n - 1 - i : i;
+    T::load(rx, x + (long)c * kChunkF32 * ro.ldx, ro.ldx, w.live - c * kChunkF32);
+    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, w.live - c * kChunkF32);
+    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, w.live - c * kChunkF32);
+  };
+  if (n) fetch(0);
+  for (int i = 0; i < n; ++i) {
+    const int c = rev ? n - 1 - i : i;
+    const int rows = min(kChunkF32, w.live - c * kChunkF32);
+    T::put(xtile, rx);
+    T::put(ytile, ry);
+    T::put(ztile, rz);
+    __syncthreads();
+    if (i + 1 < n) fetch(i + 1);
+    // every wave for itself: the pairs, and what the state gives its columns
+    f32x16 s, o;
+    s = 0.f;
+    o = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int at = t * 32 + q * 8 + hh * 4;
+        const float4 xv = *(const float4*)(xtile + li * T::LD + at);
+        const float4 yv = *(const float4*)(ytile + li * T::LD + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s = __builtin_amdgcn_mfma_f32_32x32x2f32(elem(yv, e), elem(xv, e), s, 0, 0, 0);
+          o = __builtin_amdgcn_mfma_f32_32x32x2f32(S[t][4 * q + e], elem(xv, e), o, 0, 0, 0);
+        }
+      }
+    if (have_state) o *= ro.a_state * decay_pow(w.g2, rev ? max(rows - 1 - li, 0) : li + 1);
+    float zf[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = (r >> 2) * 8 + hh * 4 + (r & 3);
+      const int far = rev ? j - li : li - j;
+      const float pair = far >= 0 ? s[r] * (ro.a_pair * decay_pow(w.g2, max(far, 0))) : 0.f;
+      zf[r] = ztile[j * T::LD + wave * 32 + li];
+      o = __builtin_amdgcn_mfma_f32_32x32x2f32(zf[r], pair, o, 0, 0, 0);
+    }
+    if (li < rows) {
+      float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunkF32 + li) * ro.ldo + (long)(w.h / ro.go) * D + wave * 32;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(float4*)(out + q * 8 + hh * 4) = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+    }
+    if (i + 1 < n || keep_last) update_state_f32<D>(S, ytile, zf, w.g2, ro.a_update, rows, rev, lane);
+    have_state = true;
+    __syncthreads();
+  }
+  if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
+  for (int k = threadIdx.x; k < (w.s1 - w.s0 - w.live) * T::UNITS; k += T::THREADS)
+    *(float4*)((float*)ro.out + ((long)w.b * p.seq + w.s0 + w.live + k / T::UNITS) * ro.ldo + (long)(w.h / ro.go) * D +
+               (k % T::UNITS) * 4) = make_float4(0, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------------------
+// gradients of shared heads: the query heads' f32 parts, [rows, heads, D], summed in their order
+// ---------------------------------------------------------------------------
+template <class E>
+__global__ __launch_bounds__(256) void linattn_group_sum_kernel(const float* parts_k, const float* parts_v, E* dk, E* dv,
+                                                                long lddk, long lddv, long rows, int kv_heads, int group,
+                                                                int dim) {
+  const float* parts = blockIdx.y ? parts_v : parts_k;
+  E* out = blockIdx.y ? dv : dk;
+  const long ld = blockIdx.y ? lddv : lddk;
+  const int per_head = dim / 4, per_row = kv_heads * per_head;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * per_row; i += (long)gridDim.x * 256) {
+    const long row = i / per_row;
+    const int c = i % per_row, h = c / per_head, e = (c % per_head) * 4;
+    const float* src = parts + (row * kv_heads + h) * (long)group * dim + e;
+    float4 s = *(const float4*)src;
+    for (int g = 1; g < group; ++g) {
+      const float4 v = *(const float4*)(src + g * dim);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    E* to = out + row * ld + h * dim + e;
+    if constexpr (sizeof(E) == 2)
+      *(uint2*)to = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
+    else
+      *(float4*)to = s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// one token per sequence: the state is read and written once and is all that counts.  A workgroup has 32
+// columns of a state: 8 threads of 16 bytes a row, 32 rows at a time.
+// ---------------------------------------------------------------------------
+template <class E>
+__device__ __forceinline__ float value(const E* p) {
+  if constexpr (sizeof(E) == 2) return bf16_to_f32(*p);
+  else return *p;
+}
+
+template <class E, int D>
+__global__ __launch_bounds__(256) void linattn_step_kernel(const E* q, const E* k, const E* v, E* o, const float* decay,
+                                                           const float* state_in, float* state_out, long ldq, long ldk,
+                                                           long ldv, long ldo, int heads, int group, float scale) {
+  constexpr int SLICES = D / 32;
+  __shared__ float4 red[4][8];
+  const int slice = blockIdx.x % SLICES;
+  const unsigned bh = blockIdx.x / SLICES;
+  const int h = bh % heads, hk = h / group, b = bh / heads;
+  const int c4 = threadIdx.x & 7, r0 = threadIdx.x >> 3, col = slice * 32 + c4 * 4;
+  const float lambda = exp2f(log2_decay(decay, h));
+  const long base = (long)bh * D * D + col;
+  const E* vp = v + b * ldv + (long)hk * D + col;
+  const float4 vv = make_float4(value(vp), value(vp + 1), value(vp + 2), value(vp + 3));
+  float4 s[D / 32], acc = make_float4(0, 0, 0, 0);
+  float kd[D / 32], qd[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    kd[i] = value(k + b * ldk + (long)hk * D + r0 + 32 * i);
+    qd[i] = value(q + b * ldq + (long)h * D + r0 + 32 * i) * scale;
+  }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+    s[i] = state_in ? *(const float4*)(state_in + base + (long)(r0 + 32 * i) * D) : make_float4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    s[i] = make_float4(lambda * s[i].x + kd[i] * vv.x, lambda * s[i].y + kd[i] * vv.y, lambda * s[i].z + kd[i] * vv.z,
+                       lambda * s[i].w + kd[i] * vv.w);
+    *(float4*)(state_out + base + (long)(r0 + 32 * i) * D) = s[i];
+    acc.x += qd[i] * s[i].x; acc.y += qd[i] * s[i].y; acc.z += qd[i] * s[i].z; acc.w += qd[i] * s[i].w;
+  }
+  // over the 8 rows of a wave, then over the waves
+#pragma unroll
+  for (int m = 8; m < 64; m <<= 1) {
+    acc.x += __shfl_xor(acc.x, m); acc.y += __shfl_xor(acc.y, m);
+    acc.z += __shfl_xor(acc.z, m); acc.w += __shfl_xor(acc.w, m);
+  }
+  if ((threadIdx.x & 63) < 8) red[threadIdx.x >> 6][c4] = acc;
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    const float4 a = red[0][c4], b4 = red[1][c4], c = red[2][c4], d = red[3][c4];
+    const float4 r = make_float4(a.x + b4.x + c.x + d.x, a.y + b4.y + c.y + d.y, a.z + b4.z + c.z + d.z,
+                                 a.w + b4.w + c.w + d.w);
+    E* to = o + b * ldo + (long)h * D + col;
+    if constexpr (sizeof(E) == 2)
+      *(uint2*)to = make_uint2(pack2(r.x, r.y), pack2(r.z, r.w));
+    else
+      *(float4*)to = r;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+constexpr int kSegUnit = 128;      // rows a segment is a multiple of
+constexpr int kWantWorkgroups = 512;
+
+// Rows of a segment for `walks` sequences x heads x roles: one segment if they fill the device, else as
+// many as bring two workgroups to a CU.
+int segment_rows(int64_t walks, int64_t seq) {
+  if (walks >= kWantWorkgroups || seq <= 2 * kSegUnit) return (int)std::max<int64_t>(seq, 1);
+  const int64_t segs = (kWantWorkgroups + walks - 1) / walks;
+  const int64_t rows = (seq + segs - 1) / segs;
+  const int64_t unit = (rows + kSegUnit - 1) / kSegUnit * kSegUnit;
+  return (int)std::min<int64_t>(unit, seq);
+}
+
+struct Split {
+  int rows, n;
+  size_t parts;        // bytes of one role's segment states
+  size_t groups;       // bytes of one gradient's query-head parts
+};
+Split split_of(const jpp_linattn_args* a, int roles) {
+  Split s;
+  s.rows = segment_rows((int64_t)a->batch * a->n_heads * roles, a->seq);
+  s.n = std::max(1, (a->seq + s.rows - 1) / s.rows);     // (no rows: a walk that hands the state on)
+  const size_t states = (size_t)a->batch * a->n_heads * a->head_dim * a->head_dim * 4;
+  s.parts = s.n > 1 ? states * s.n : 0;
+  s.groups = roles > 1 && a->n_kv_heads < a->n_heads ? (size_t)a->batch * a->seq * a->n_heads * a->head_dim * 4 : 0;
+  return s;
+}
+
+int check_sizes(const jpp_linattn_args* a, const char* who) {
+  JPP_REQUIRE(a, "%s: null operand", who);
+  JPP_REQUIRE(a->dtype == JPP_DTYPE_BF16 || a->dtype == JPP_DTYPE_F32, "%s: dtype %d", who, a->dtype);
+  JPP_REQUIRE(a->batch >= 0 && a->seq >= 0, "%s: batch %d, seq %d", who, a->batch, a->seq);
+  JPP_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "%s: head_dim %d (64 or 128)", who, a->head_dim);
+  JPP_REQUIRE(a->n_heads > 0 && a->n_kv_heads > 0 && a->n_heads % a->n_kv_heads == 0, "%s: %d heads on %d", who, a->n_heads,
+              a->n_kv_heads);
+  // (a launch has less than 2^32 threads; the kernels count a sequence's rows in int)
+  JPP_REQUIRE((int64_t)a->batch * a->n_heads < (1 << 22) && a->seq < (1 << 30),
+              "%s: batch %d x %d heads x %d rows are too many", who, a->batch, a->n_heads, a->seq);
+  return JPP_OK;
+}
+
+int check_tensor(const void* p, int64_t ld, int heads, int rows, const jpp_linattn_args* a, const char* who,
+                 const char* name) {
+  const int unit = a->dtype == JPP_DTYPE_F32 ? 4 : 8;
+  if (rows == 0) return JPP_OK;      // nothing of it is touched
+  JPP_REQUIRE(p, "%s: null operand %s", who, name);
+  JPP_REQUIRE(ld >= (int64_t)heads * a->head_dim, "%s: leading dimension of %s too small", who, name);
+  JPP_REQUIRE(ld % unit == 0 && (uintptr_t)p % 16 == 0, "%s: %s must keep 16-byte alignment", who, name);
+  return JPP_OK;
+}
+int check_state(const void* p, const char* who, const char* name) {
+  JPP_REQUIRE((uintptr_t)p % 16 == 0, "%s: %s must be 16-byte aligned", who, name);
+  return JPP_OK;
+}
+
+#define JPP_TRY(expr)             \
+  do {                            \
+    if (int rc_ = (expr)) return rc_; \
+  } while (0)
+
+template <int D, bool F32>
+int launch(hipStream_t st, const Params& p) {
+  const int64_t walks = (int64_t)p.batch * p.heads * p.n_roles;
+  if (p.n_seg > 1) {
+    const unsigned carry = (unsigned)(walks * (D * D / 1024));
+    if constexpr (F32) hipLaunchKernelGGL((linattn_sum_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), 0, st, p);
+    else hipLaunchKernelGGL((linattn_sum_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), 0, st, p);
+    JPP_LAUNCH_CHECK();
+    hipLaunchKernelGGL((linattn_carry_kernel<D>), dim3(carry), dim3(256), 0, st, p);
+    JPP_LAUNCH_CHECK();
+  }
+  if constexpr (F32) {
+    hipLaunchKernelGGL((linattn_walk_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), 0, st, p);
+  } else {
+    constexpr int kLds = 3 * Tile<D>::BYTES + 2 * 8192;
+    if (kLds > 64 * 1024) JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D>, kLds));
+    hipLaunchKernelGGL((linattn_walk_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), kLds, st, p);
+  }
+  JPP_LAUNCH_CHECK();
+  return JPP_OK;
+}
+int launch_any(hipStream_t st, const Params& p, const jpp_linattn_args* a) {
+  const bool f32 = a->dtype == JPP_DTYPE_F32;
+  if (a->head_dim == 64) return f32 ? launch<64, true>(st, p) : launch<64, false>(st, p);
+  return f32 ? launch<128, true>(st, p) : launch<128, false>(st, p);
+}
+
+Params params_of(const jpp_linattn_args* a, const Split& s) {
+  Params p = {};
+  p.decay = a->decay;
+  p.lens = a->lens;
+  p.batch = a->batch;
+  p.seq = a->seq;
+  p.heads = a->n_heads;
+  p.n_seg = s.n;
+  p.seg_rows = s.rows;
+  return p;
+}
+
+double flops_of(const jpp_linattn_args* a) {
+  return 2.0 * a->batch * a->seq * (double)a->n_heads * a->head_dim * a->head_dim;
+}
+
+}  // namespace
+
+extern "C" size_t jpp_linattn_workspace_bytes(const jpp_linattn_args* a, int backward) {
+  if (check_sizes(a, "linattn_workspace_bytes") || a->batch == 0 || a->seq == 0) return 0;
+  const Split s = split_of(a, backward ? 3 : 1);
+  return backward ? 3 * s.parts + 2 * s.groups : s.parts;
+}
+
+extern "C" int jpp_linattn_fwd(void* stream, const jpp_linattn_args* a) {
+  const char* who = "linattn_fwd";
+  JPP_TRY(check_sizes(a, who));
+  if (a->batch == 0) return JPP_OK;
+  JPP_TRY(check_tensor(a->q, a->ldq, a->n_heads, a->seq, a, who, "q"));
+  JPP_TRY(check_tensor(a->k, a->ldk, a->n_kv_heads, a->seq, a, who, "k"));
+  JPP_TRY(check_tensor(a->v, a->ldv, a->n_kv_heads, a->seq, a, who, "v"));
+  JPP_TRY(check_tensor(a->o, a->ldo, a->n_heads, a->seq, a, who, "o"));
+  JPP_REQUIRE(a->decay, "%s: null operand decay", who);
+  JPP_REQUIRE(!a->o || (a->o != a->q && a->o != a->k && a->o != a->v), "%s: o overlaps an input", who);
+  JPP_TRY(check_state(a->state_in, who, "state_in"));
+  JPP_TRY(check_state(a->state_out, who, "state_out"));
+  const Split s = split_of(a, 1);
+  JPP_REQUIRE(s.parts == 0 || a->workspace, "%s: workspace of %zu bytes wanted", who, s.parts);
+  JPP_TRY(check_state(a->workspace, who, "workspace"));
+  const int group = a->n_heads / a->n_kv_heads;
+  Params p = params_of(a, s);
+  p.n_roles = 1;
+  p.role[0] = {a->q, a->k, a->v, a->o, a->ldq, a->ldk, a->ldv, a->ldo, 1, group, group, 1, 0, 0, 0,
+               a->scale, a->scale, 1.f, a->state_in, a->state_out, (float*)a->workspace};
+  const double es = a->dtype == JPP_DTYPE_F32 ? 4 : 2;
+  ProbeScope probe((hipStream_t)stream, "linattn_fwd", 2 * flops_of(a),
+                   es * a->batch * a->seq * a->head_dim * 2.0 * (a->n_heads + a->n_kv_heads));
+  return launch_any((hipStream_t)stream, p, a);
+}
+
+extern "C" int jpp_linattn_bwd(void* stream, const jpp_linattn_args* a) {
+  const char* who = "linattn_bwd";
+  JPP_TRY(check_sizes(a, who));
+  if (a->batch == 0) return JPP_OK;
+  JPP_TRY(check_tensor(a->q, a->ldq, a->n_heads, a->seq, a, who, "q"));
+  JPP_TRY(check_tensor(a->k, a->ldk, a->n_kv_heads, a->seq, a, who, "k"));
+  JPP_TRY(check_tensor(a->v, a->ldv, a->n_kv_heads, a->seq, a, who, "v"));
+  JPP_TRY(check_tensor(a->d_o, a->lddo, a->n_heads, a->seq, a, who, "d_o"));
+  JPP_TRY(check_tensor(a->dq, a->lddq, a->n_heads, a->seq, a, who, "dq"));
+  JPP_TRY(check_tensor(a->dk, a->lddk, a->n_kv_heads, a->seq, a, who, "dk"));
+  JPP_TRY(check_tensor(a->dv, a->lddv, a->n_kv_heads, a->seq, a, who, "dv"));
+  JPP_REQUIRE(a->decay, "%s: null operand decay", who);
+  for (const void* out : {a->dq, a->dk, a->dv})
+    for (const void* in : {a->q, a->k, a->v, a->d_o}) JPP_REQUIRE(!out || out != in, "%s: a gradient overlaps an input", who);
+  JPP_REQUIRE(a->seq == 0 || (a->dq != a->dk && a->dk != a->dv && a->dq != a->dv), "%s: gradients overlap each other", who);
+  JPP_TRY(check_state(a->state_in, who, "state_in"));
+  JPP_TRY(check_state(a->d_state_out, who, "d_state_out"));
+  JPP_TRY(check_state(a->d_state_in, who, "d_state_in"));
+  // (dq's walk reads state_in and dk's d_state_out while dv's writes d_state_in)
+  JPP_REQUIRE(!a->d_state_in || (a->d_state_in != a->state_in && a->d_state_in != a->d_state_out),
+              "%s: d_state_in overlaps an input", who);
+  const Split s = split_of(a, 3);
+  JPP_REQUIRE(s.parts + s.groups == 0 || a->workspace, "%s: workspace of %zu bytes wanted", who, 3 * s.parts + 2 * s.groups);
+  JPP_TRY(check_state(a->workspace, who, "workspace"));
+  const int group = a->n_heads / a->n_kv_heads, f32 = a->dtype == JPP_DTYPE_F32;
+  const long wide = (long)a->n_heads * a->head_dim;
+  uint8_t* ws = (uint8_t*)a->workspace;
+  float* parts[3];
+  for (int i = 0; i < 3; ++i) parts[i] = (float*)(ws + i * s.parts);
+  float* dk_parts = (float*)(ws + 3 * s.parts);
+  float* dv_parts = (float*)(ws + 3 * s.parts + s.groups);
+  const bool shared = s.groups != 0;
+  Params p = params_of(a, s);
+  p.n_roles = 3;
+  p.role[0] = {a->d_o, a->v, a->k, a->dq, a->lddo, a->ldv, a->ldk, a->lddq, 1, group, group, 1, 0, 1, 0,
+               a->scale, a->scale, 1.f, a->state_in, nullptr, parts[0]};
+  p.role[1] = {a->v, a->d_o, a->q, shared ? (void*)dk_parts : a->dk, a->ldv, a->lddo, a->ldq, shared ? wide : (long)a->lddk,
+               group, 1, 1, 1, 1, 1, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, nullptr, parts[1]};
+  p.role[2] = {a->k, a->q, a->d_o, shared ? (void*)dv_parts : a->dv, a->ldk, a->ldq, a->lddo, shared ? wide : (long)a->lddv,
+               group, 1, 1, 1, 1, 0, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, a->d_state_in, parts[2]};
+  hipStream_t st = (hipStream_t)stream;
+  const double es = f32 ? 4 : 2;
+  ProbeScope probe(st, "linattn_bwd", 5 * flops_of(a),
+                   es * a->batch * a->seq * a->head_dim * (3.0 * a->n_heads + 4.0 * a->n_kv_heads));
+  JPP_TRY(launch_any(st, p, a));
+  if (shared) {
+    const long rows = (long)a->batch * a->seq;
+    const long units = rows * a->n_kv_heads * (a->head_dim / 4);
+    const dim3 grid((unsigned)std::min<long>((units + 255) / 256, 1 << 20), 2);
+    if (f32)
+      hipLaunchKernelGGL((linattn_group_sum_kernel<float>), grid, dim3(256), 0, st, dk_parts, dv_parts, (float*)a->dk,
+                         (float*)a->dv, a->lddk, a->lddv, rows, a->n_kv_heads, group, a->head_dim);
+    else
+      hipLaunchKernelGGL((linattn_group_sum_kernel<bf16_t>), grid, dim3(256), 0, st, dk_parts, dv_parts, (bf16_t*)a->dk,
+                         (bf16_t*)a->dv, a->lddk, a->lddv, rows, a->n_kv_heads, group, a->head_dim);
+    JPP_LAUNCH_CHECK();
+  }
+  return JPP_OK;
+}
+
+extern "C" int jpp_linattn_step(void* stream, const jpp_linattn_args* a) {
+  const char* who = "linattn_step";
+  JPP_TRY(check_sizes(a, who));
+  if (a->batch == 0) return JPP_OK;
+  JPP_TRY(check_tensor(a->q, a->ldq, a->n_heads, 1, a, who, "q"));
+  JPP_TRY(check_tensor(a->k, a->ldk, a->n_kv_heads, 1, a, who, "k"));
+  JPP_TRY(check_tensor(a->v, a->ldv, a->n_kv_heads, 1, a, who, "v"));
+  JPP_TRY(check_tensor(a->o, a->ldo, a->n_heads, 1, a, who, "o"));
+  JPP_REQUIRE(a->decay && a->state_out, "%s: null operand", who);
+  JPP_REQUIRE(!a->o || (a->o != a->q && a->o != a->k && a->o != a->v), "%s: o overlaps an input", who);
+  JPP_TRY(check_state(a->state_in, who, "state_in"));
+  JPP_TRY(check_state(a->state_out, who, "state_out"));
+  hipStream_t st = (hipStream_t)stream;
+  const int group = a->n_heads / a->n_kv_heads;
+  const dim3 grid((unsigned)(a->batch * (int64_t)a->n_heads * (a->head_dim / 32)));
+  ProbeScope probe(st, "linattn_step", 4.0 * a->batch * a->n_heads * a->head_dim * (double)a->head_dim,
+                   8.0 * a->batch * a->n_heads * a->head_dim * (double)a->head_dim);
+#define JPP_STEP(E_, D_)                                                                                              \
+  hipLaunchKernelGGL((linattn_step_kernel<E_, D_>), grid, dim3(256), 0, st, (const E_*)a->q, (const E_*)a->k,         \
+                     (const E_*)a->v, (E_*)a->o, a->decay, a->state_in, a->state_out, a->ldq, a->ldk, a->ldv, a->ldo, \
+                     a->n_heads, group, a->scale)
+  if (a->dtype == JPP_DTYPE_F32) {
+    if (a->head_dim == 64) JPP_STEP(float, 64); else JPP_STEP(float, 128);
+  } else {
+    if (a->head_dim == 64) JPP_STEP(bf16_t, 64); else JPP_STEP(bf16_t, 128);
+  }
+#undef JPP_STEP
+  JPP_LAUNCH_CHECK();
+  return JPP_OK;
+}

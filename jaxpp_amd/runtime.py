@@ -86,6 +86,35 @@ class ColsumItem(C.Structure):
     _fields_ = [("x", C.c_void_p), ("ld", C.c_int64), ("cols", C.c_int64), ("acc", C.c_void_p)]
 
 
+class LinattnArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("d_o", C.c_void_p),
+                ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("decay", C.c_void_p),
+                ("state_in", C.c_void_p), ("state_out", C.c_void_p), ("d_state_out", C.c_void_p),
+                ("d_state_in", C.c_void_p), ("lens", C.c_void_p), ("workspace", C.c_void_p),
+                ("ldq", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64), ("ldo", C.c_int64),
+                ("lddo", C.c_int64), ("lddq", C.c_int64), ("lddk", C.c_int64), ("lddv", C.c_int64),
+                ("batch", C.c_int), ("seq", C.c_int), ("n_heads", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("scale", C.c_float), ("dtype", C.c_int)]
+
+
+class JoinArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("b", C.c_void_p), ("gamma_post", C.c_void_p), ("gate", C.c_void_p),
+                ("gamma_pre", C.c_void_p), ("h", C.c_void_p), ("y", C.c_void_p), ("rstd_post", C.c_void_p),
+                ("rstd_pre", C.c_void_p), ("dh", C.c_void_p), ("dy", C.c_void_p), ("dx", C.c_void_p),
+                ("db", C.c_void_p), ("dgamma_post", C.c_void_p), ("dgate", C.c_void_p),
+                ("dgamma_pre", C.c_void_p), ("workspace", C.c_void_p), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("gate_rows", C.c_int64), ("alpha", C.c_float), ("eps", C.c_float),
+                ("accumulate", C.c_int), ("dtype", C.c_int)]
+
+
+class DistillArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ids", C.c_void_p), ("teacher", C.c_void_p), ("weight", C.c_void_p),
+                ("row_loss", C.c_void_p), ("loss", C.c_void_p), ("dlogits", C.c_void_p), ("workspace", C.c_void_p),
+                ("ld", C.c_int64),
+                ("ldd", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int64), ("k", C.c_int),
+                ("temperature", C.c_float), ("scale", C.c_float), ("dtype", C.c_int)]
+
+
 class StageDesc(C.Structure):
     _fields_ = [("family", C.c_int), ("hidden", C.c_int), ("n_heads", C.c_int),
                 ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("ffn", C.c_int),
@@ -122,7 +151,8 @@ EXPORTS = [
     "jpp_norm_fwd", "jpp_norm_bwd", "jpp_norm_bwd_static", "jpp_swiglu_fwd", "jpp_swiglu_bwd", "jpp_rope",
     "jpp_grad_accum_f32", "jpp_sum_accum_f32", "jpp_colsum_accum", "jpp_colsum_accum_multi", "jpp_mse_loss", "jpp_moe_capacity", "jpp_moe_route",
     "jpp_moe_gather", "jpp_moe_combine_fwd", "jpp_moe_bwd_prepare", "jpp_moe_combine_bwd",
-    "jpp_moe_router_wgrad", "jpp_cast_f32_to_bf16", "jpp_cast_bf16_to_f32", "jpp_adam_step",
+    "jpp_moe_router_wgrad", "jpp_linattn_workspace_bytes", "jpp_linattn_fwd", "jpp_linattn_bwd", "jpp_linattn_step",
+    "jpp_block_join_fwd", "jpp_block_join_bwd", "jpp_distill_loss", "jpp_cast_f32_to_bf16", "jpp_cast_bf16_to_f32", "jpp_adam_step",
     "jpp_stage_optimizer_init", "jpp_stage_opt_ptr", "jpp_stage_adam_step",
     "jpp_stage_create", "jpp_stage_destroy", "jpp_stage_n_params", "jpp_stage_param_info",
     "jpp_stage_param_ptr", "jpp_stage_grad_ptr", "jpp_stage_zero_grads", "jpp_stage_join",
@@ -241,6 +271,13 @@ def load():
                                          C.c_void_p, C.c_void_p]
     lib.jpp_cast_f32_to_bf16.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]
     lib.jpp_cast_bf16_to_f32.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]
+    lib.jpp_linattn_workspace_bytes.restype = C.c_size_t
+    lib.jpp_linattn_workspace_bytes.argtypes = [C.POINTER(LinattnArgs), C.c_int]
+    for name in ("fwd", "bwd", "step"):
+        getattr(lib, "jpp_linattn_" + name).argtypes = [C.c_void_p, C.POINTER(LinattnArgs)]
+    for name in ("fwd", "bwd"):
+        getattr(lib, "jpp_block_join_" + name).argtypes = [C.c_void_p, C.POINTER(JoinArgs)]
+    lib.jpp_distill_loss.argtypes = [C.c_void_p, C.POINTER(DistillArgs)]
     lib.jpp_stage_create.argtypes = [C.POINTER(StageDesc), C.POINTER(C.c_void_p)]
     lib.jpp_stage_destroy.argtypes = [C.c_void_p]
     lib.jpp_stage_n_params.argtypes = [C.c_void_p]
@@ -614,6 +651,69 @@ def adam_step(count, grad, m, v, step, master=None, param=None, lr=1e-3, b1=0.9,
     a = AdamArgs(count, grad, master, param, m, v, step, lr, b1, b2, eps, grad_scale,
                  int(zero_grad))
     check(load().jpp_adam_step(stream, C.byref(a)))
+
+
+def linattn_workspace(batch, seq, n_heads, n_kv_heads, head_dim, backward=False, f32=False) -> int:
+    """Bytes of scratch of `linattn_fwd`, or of `linattn_bwd`."""
+    a = LinattnArgs(batch=batch, seq=seq, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, dtype=int(f32))
+    return load().jpp_linattn_workspace_bytes(C.byref(a), int(backward))
+
+
+def linattn_fwd(q, k, v, o, decay, ldq, ldk, ldv, ldo, batch, seq, n_heads, n_kv_heads, head_dim, scale, state_in=None,
+                state_out=None, lens=None, workspace=None, f32=False, stream=None):
+    """Linear attention with a decay for each head (jpp_linattn_fwd)."""
+    a = LinattnArgs(q=q, k=k, v=v, o=o, decay=decay, state_in=state_in, state_out=state_out, lens=lens,
+                    workspace=workspace, ldq=ldq, ldk=ldk, ldv=ldv, ldo=ldo, batch=batch, seq=seq, n_heads=n_heads,
+                    n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale, dtype=int(f32))
+    check(load().jpp_linattn_fwd(stream, C.byref(a)))
+
+
+def linattn_bwd(q, k, v, d_o, dq, dk, dv, decay, ldq, ldk, ldv, lddo, lddq, lddk, lddv, batch, seq, n_heads, n_kv_heads,
+                head_dim, scale, state_in=None, d_state_out=None, d_state_in=None, lens=None, workspace=None, f32=False,
+                stream=None):
+    """Its gradients (jpp_linattn_bwd)."""
+    a = LinattnArgs(q=q, k=k, v=v, d_o=d_o, dq=dq, dk=dk, dv=dv, decay=decay, state_in=state_in,
+                    d_state_out=d_state_out, d_state_in=d_state_in, lens=lens, workspace=workspace, ldq=ldq, ldk=ldk,
+                    ldv=ldv, lddo=lddo, lddq=lddq, lddk=lddk, lddv=lddv, batch=batch, seq=seq, n_heads=n_heads,
+                    n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale, dtype=int(f32))
+    check(load().jpp_linattn_bwd(stream, C.byref(a)))
+
+
+def linattn_step(q, k, v, o, decay, state_in, state_out, ldq, ldk, ldv, ldo, batch, n_heads, n_kv_heads, head_dim, scale,
+                 f32=False, stream=None):
+    """One token per sequence (jpp_linattn_step); `state_out` may be `state_in`."""
+    a = LinattnArgs(q=q, k=k, v=v, o=o, decay=decay, state_in=state_in, state_out=state_out, ldq=ldq, ldk=ldk, ldv=ldv,
+                    ldo=ldo, batch=batch, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale,
+                    dtype=int(f32))
+    check(load().jpp_linattn_step(stream, C.byref(a)))
+
+
+def block_join_fwd(x, b, h, rows, cols, y=None, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None, rstd_post=None,
+                   rstd_pre=None, alpha=1.0, eps=1e-6, f32=False, stream=None):
+    """A block's output joined to the residual stream: norm, gate, residual scale, next norm (jpp_block_join_fwd)."""
+    a = JoinArgs(x=x, b=b, gamma_post=gamma_post, gate=gate, gamma_pre=gamma_pre, h=h, y=y, rstd_post=rstd_post,
+                 rstd_pre=rstd_pre, rows=rows, cols=cols, gate_rows=gate_rows, alpha=alpha, eps=eps, dtype=int(f32))
+    check(load().jpp_block_join_fwd(stream, C.byref(a)))
+
+
+def block_join_bwd(h, b, dh, dy, dx, db, rows, cols, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None,
+                   rstd_post=None, rstd_pre=None, dgamma_post=None, dgate=None, dgamma_pre=None, workspace=None,
+                   alpha=1.0, accumulate=True, f32=False, stream=None):
+    """Its gradients (jpp_block_join_bwd); the sums over rows are added to what is there if `accumulate`."""
+    a = JoinArgs(b=b, gamma_post=gamma_post, gate=gate, gamma_pre=gamma_pre, h=h, rstd_post=rstd_post, rstd_pre=rstd_pre,
+                 dh=dh, dy=dy, dx=dx, db=db, dgamma_post=dgamma_post, dgate=dgate, dgamma_pre=dgamma_pre,
+                 workspace=workspace, rows=rows, cols=cols, gate_rows=gate_rows, alpha=alpha, accumulate=int(accumulate),
+                 dtype=int(f32))
+    check(load().jpp_block_join_bwd(stream, C.byref(a)))
+
+
+def distill_loss(logits, ids, teacher, rows, vocab, k, ld, row_loss, loss=None, dlogits=None, ldd=0, weight=None,
+                 temperature=1.0, scale=1.0, workspace=None, f32=False, stream=None):
+    """Loss and gradient of logits against a teacher's top logits (jpp_distill_loss)."""
+    a = DistillArgs(logits=logits, ids=ids, teacher=teacher, weight=weight, row_loss=row_loss, loss=loss,
+                    dlogits=dlogits, workspace=workspace, ld=ld, ldd=ldd, rows=rows, vocab=vocab, k=k, temperature=temperature, scale=scale,
+                    dtype=int(f32))
+    check(load().jpp_distill_loss(stream, C.byref(a)))
 
 
 # Elements of tensors that travel in one call, or one larger tensor (of a layer's results, the layer): what bounds the

@@ -1,0 +1,164 @@
+"""Plain float64 restatements of the operators of a linear-attention student: linear attention with a
+decay for each head, the join of a block to the residual stream, the distillation loss.  Test
+infrastructure only; written from the definitions, every row (or pair of rows) for itself."""
+from __future__ import annotations
+
+import numpy as np
+
+
+# ---------------------------------------------------------------------------
+# linear attention
+# ---------------------------------------------------------------------------
+def linattn_recurrence(q, k, v, decay, scale, state=None, lens=None):
+    """q [b, t, h, d], k, v [b, t, hk, d], decay [h] (logarithms) -> o, final state [b, h, d, d]; token by
+    token."""
+    q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
+    b, t, h, d = q.shape
+    group = h // k.shape[2]
+    s = np.zeros((b, h, d, d)) if state is None else np.array(state, np.float64)
+    o = np.zeros((b, t, h, d))
+    lens = [t] * b if lens is None else [min(max(int(n), 0), t) for n in lens]
+    lam = np.exp(np.asarray(decay, np.float64))[:, None, None]
+    for ib in range(b):
+        for it in range(lens[ib]):
+            kk, vv = k[ib, it].repeat(group, 0), v[ib, it].repeat(group, 0)
+            s[ib] = lam * s[ib] + kk[:, :, None] * vv[:, None, :]
+            o[ib, it] = scale * np.matmul(q[ib, it][:, None, :], s[ib])[:, 0]
+    return o, s
+
+
+def _powers(decay, n):
+    """lambda ** n for n >= 0, with lambda ** 0 = 1 also where the logarithm is -inf."""
+    with np.errstate(invalid="ignore"):
+        return np.where(n == 0, 1.0, np.exp(np.where(n == 0, 0.0, decay * np.maximum(n, 0))))
+
+
+def linattn(q, k, v, decay, scale, state=None, lens=None):
+    """The same by pairs of rows."""
+    q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
+    b, t, h, d = q.shape
+    group = h // k.shape[2]
+    o, s = np.zeros((b, t, h, d)), np.zeros((b, h, d, d))
+    for ib in range(b):
+        n = t if lens is None else min(max(int(lens[ib]), 0), t)
+        at = np.arange(n)
+        for ih in range(h):
+            g, qq, kk, vv = float(decay[ih]), q[ib, :n, ih], k[ib, :n, ih // group], v[ib, :n, ih // group]
+            w = np.where(at[:, None] >= at[None, :], _powers(g, at[:, None] - at[None, :]), 0.0)
+            o[ib, :n, ih] = scale * ((qq @ kk.T) * w) @ vv
+            s[ib, ih] = (kk * _powers(g, n - 1 - at)[:, None]).T @ vv
+            if state is not None:
+                s0 = np.asarray(state[ib, ih], np.float64)
+                o[ib, :n, ih] += scale * _powers(g, at + 1)[:, None] * (qq @ s0)
+                s[ib, ih] += _powers(g, np.array(n)) * s0
+    return o, s
+
+
+def linattn_bwd(q, k, v, d_o, decay, scale, state=None, d_state=None, lens=None):
+    """Gradients of sum(o * d_o) + sum(final state * d_state): dq, dk, dv, d(initial state)."""
+    q, k, v, d_o = (np.asarray(a, np.float64) for a in (q, k, v, d_o))
+    b, t, h, d = q.shape
+    group = h // k.shape[2]
+    dq, dk, dv = np.zeros_like(q), np.zeros_like(k), np.zeros_like(v)
+    ds = np.zeros((b, h, d, d))
+    for ib in range(b):
+        n = t if lens is None else min(max(int(lens[ib]), 0), t)
+        at = np.arange(n)
+        for ih in range(h):
+            ik, g = ih // group, float(decay[ih])
+            qq, kk, vv, oo = q[ib, :n, ih], k[ib, :n, ik], v[ib, :n, ik], d_o[ib, :n, ih]
+            w = scale * np.where(at[:, None] >= at[None, :], _powers(g, at[:, None] - at[None, :]), 0.0)
+            pairs, d_pairs = (qq @ kk.T) * w, (oo @ vv.T) * w
+            dq[ib, :n, ih] = d_pairs @ kk
+            dk[ib, :n, ik] += d_pairs.T @ qq
+            dv[ib, :n, ik] += pairs.T @ oo
+            down, up = _powers(g, at + 1)[:, None], _powers(g, n - 1 - at)[:, None]
+            ds[ib, ih] = scale * (qq * down).T @ oo
+            if state is not None:
+                dq[ib, :n, ih] += scale * down * (oo @ np.asarray(state[ib, ih], np.float64).T)
+            if d_state is not None:
+                u = np.asarray(d_state[ib, ih], np.float64)
+                dk[ib, :n, ik] += up * (vv @ u.T)
+                dv[ib, :n, ik] += up * (kk @ u)
+                ds[ib, ih] += _powers(g, np.array(n)) * u
+    return dq, dk, dv, ds
+
+
+# ---------------------------------------------------------------------------
+# block join
+# ---------------------------------------------------------------------------
+def _gate(gate, gate_rows, rows):
+    return 1.0 if gate is None else np.repeat(np.asarray(gate, np.float64), gate_rows, axis=0)[:rows]
+
+
+def block_join(x, b, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None, alpha=1.0, eps=1e-6):
+    x, b = np.asarray(x, np.float64), np.asarray(b, np.float64)
+    out = {}
+    n = b
+    if gamma_post is not None:
+        out["rstd_post"] = 1.0 / np.sqrt(np.mean(b * b, 1) + eps)
+        n = b * out["rstd_post"][:, None] * np.asarray(gamma_post, np.float64)
+    out["h"] = alpha * x + _gate(gate, gate_rows, x.shape[0]) * n
+    if gamma_pre is not None:
+        out["rstd_pre"] = 1.0 / np.sqrt(np.mean(out["h"] ** 2, 1) + eps)
+        out["y"] = out["h"] * out["rstd_pre"][:, None] * np.asarray(gamma_pre, np.float64)
+    return out
+
+
+def block_join_bwd(h, b, dh, dy, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None, rstd_post=None,
+                   rstd_pre=None, alpha=1.0):
+    """With the statistics as given (so that a rounded h is taken for what it is)."""
+    b = np.asarray(b, np.float64)
+    rows, cols = b.shape
+    total = np.zeros_like(b) if dh is None else np.array(dh, np.float64)
+    out = {}
+    if gamma_pre is not None:
+        dy, hat = np.asarray(dy, np.float64), np.asarray(h, np.float64) * np.asarray(rstd_pre, np.float64)[:, None]
+        t = dy * np.asarray(gamma_pre, np.float64)
+        total += np.asarray(rstd_pre, np.float64)[:, None] * (t - hat * np.mean(t * hat, 1, keepdims=True))
+        out["dgamma_pre"] = (dy * hat).sum(0)
+    out["dx"] = alpha * total
+    g = _gate(gate, gate_rows, rows)
+    if gamma_post is not None:
+        r = np.asarray(rstd_post, np.float64)[:, None]
+        gp, hat = np.asarray(gamma_post, np.float64), b * np.asarray(rstd_post, np.float64)[:, None]
+        u = total * g * gp
+        out["db"] = r * (u - hat * np.mean(u * hat, 1, keepdims=True))
+        out["dgamma_post"] = (total * g * hat).sum(0)
+        n = hat * gp
+    else:
+        out["db"] = total * g
+        n = b
+    if gate is not None:
+        out["dgate"] = (total * n).reshape(-1, gate_rows, cols).sum(1)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# distillation
+# ---------------------------------------------------------------------------
+def distill(logits, ids, teacher, weight=None, temperature=1.0, scale=1.0):
+    """-> row_loss, loss, dlogits.  Rows that carry nothing (weight 0, no listed teacher logit above -inf, no
+    student logit above -inf) are zero."""
+    logits = np.asarray(logits, np.float64)
+    rows, vocab = logits.shape
+    row_loss, grad = np.zeros(rows), np.zeros((rows, vocab))
+    for r in range(rows):
+        w = 1.0 if weight is None else float(weight[r])
+        listed = [(int(i), float(t)) for i, t in zip(ids[r], teacher[r]) if 0 <= i < vocab]
+        if w == 0 or not any(t > -np.inf for _, t in listed) or not (logits[r] > -np.inf).any():
+            continue
+        at = np.array([i for i, _ in listed])
+        t = np.array([t for _, t in listed]) / temperature
+        log_p = t - t.max()
+        log_p = log_p - np.log(np.exp(log_p).sum())
+        z = logits[r] / temperature
+        log_q = z - z.max()
+        log_q = log_q - np.log(np.exp(log_q).sum())
+        p = np.exp(log_p)
+        some = p > 0
+        row_loss[r] = w * temperature ** 2 * (p[some] * (log_p[some] - log_q[at][some])).sum()
+        d = np.exp(log_q)
+        np.add.at(d, at, -p)
+        grad[r] = scale * w * temperature * d
+    return row_loss, scale * row_loss.sum(), grad

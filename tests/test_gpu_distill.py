@@ -1,0 +1,206 @@
+"""The distillation loss on the GPU, against the float64 restatement.
+
+Tolerances.  log q and log p are differences of f32 values as large as M = max |z| / T + log(vocab), in units of 2^-24 of
+it, with an exponential's argument and result rounded likewise: an absolute error of 2^-21 M in each, and as much
+relative in q and p.  So a row's loss is within w T^2 2^-20 M, its gradient within scale w T (q + p) 2^-20 M (and half a
+unit in the last place where it is bf16; a whole one, 2^-8, is granted)."""
+import numpy as np
+import pytest
+
+from jaxpp_amd import runtime as rt
+from oracle import student as O
+from oracle.layers import bf16_round
+
+pytestmark = pytest.mark.gpu
+SHARE, ULP = 2.0 ** -20, 2.0 ** -8
+
+
+class Problem:
+    def __init__(self, rows, vocab, k, f32=False, temperature=1.0, pad=0, pad_out=None, seed=0, scale=0.37, weights=True):
+        rng = np.random.default_rng(seed + rows * 1000003 + vocab)
+        z = (3 * rng.standard_normal((rows, vocab))).astype(np.float32)
+        self.z = z if f32 else bf16_round(z)
+        self.f32, self.t, self.scale = f32, temperature, scale
+        self.ld, self.ldd = vocab + pad, vocab + (pad if pad_out is None else pad_out)
+        k_each = min(k, vocab)
+        self.ids = np.full((rows, k), -1, np.int32)
+        for r in range(rows):
+            self.ids[r, :k_each] = rng.choice(vocab, k_each, replace=False)
+        self.teacher = (8 + 2 * rng.standard_normal((rows, k))).astype(np.float32)
+        self.w = rng.uniform(0.5, 1.5, rows).astype(np.float32) if weights else None
+
+    def _rows(self, a, ld):
+        full = np.full((a.shape[0], ld), np.nan, np.float32)
+        full[:, :a.shape[1]] = a
+        return rt.DeviceBuffer.from_numpy(full if self.f32 else rt.to_bf16_bits(full))
+
+    def run(self, in_place=False, grad=True, workspace=True, stream=None):
+        rows, vocab = self.z.shape
+        z = self._rows(self.z, self.ld)
+        dz = None if not grad else z if in_place else self._rows(np.full(self.z.shape, 5.0), self.ldd)
+        ids, teacher = rt.DeviceBuffer.from_numpy(self.ids), rt.DeviceBuffer.from_numpy(self.teacher)
+        w = None if self.w is None else rt.DeviceBuffer.from_numpy(self.w)
+        row_loss, loss = rt.DeviceBuffer(4 * rows), rt.DeviceBuffer(4)
+        need = rt.load().jpp_workspace_bytes(8, rows, 0, 0)
+        ws = rt.DeviceBuffer.from_numpy(np.full(need // 4 + 16, np.nan, np.float32))
+        rt.distill_loss(z.ptr, ids.ptr, teacher.ptr, rows, vocab, self.ids.shape[1], self.ld, row_loss.ptr, loss=loss.ptr,
+                        dlogits=dz.ptr if grad else None, ldd=self.ldd, weight=w.ptr if w else None, temperature=self.t,
+                        scale=self.scale, workspace=ws.ptr if workspace else None, f32=self.f32, stream=stream)
+        rt.sync()
+        assert np.isnan(ws.download(np.float32, (16,), need)).all(), "wrote behind the workspace"
+        d = None
+        if grad:
+            full = dz.download(np.float32 if self.f32 else np.uint16, (rows, self.ldd))
+            full = full if self.f32 else rt.from_bf16_bits(full)
+            assert np.isnan(full[:, vocab:]).all(), "wrote behind a row"
+            d = full[:, :vocab]
+        return row_loss.download(np.float32, (rows,)), float(loss.download(np.float32, (1,))[0]), d
+
+    def check(self, **kw):
+        row, loss, d = self.run(**kw)
+        want_row, want_loss, want_d = O.distill(self.z, self.ids, self.teacher, self.w, self.t, self.scale)
+        rows, vocab = self.z.shape
+        finite = np.where(np.isfinite(self.z) & (self.z > -1e30), np.abs(self.z), 0).max(1)
+        taught = np.where(np.isfinite(self.teacher), np.abs(self.teacher), 0).max(1)
+        m = np.maximum(finite, taught) / self.t + np.log(vocab) + 1
+        w = np.ones(rows) if self.w is None else np.abs(self.w)
+        with np.errstate(invalid="ignore"):
+            off = np.where(row == want_row, 0, np.abs(row - want_row))
+        bound = SHARE * w * self.t ** 2 * m + 1e-30
+        assert (off <= bound).all(), f"row_loss: {np.max(off / bound):.3g} x the bound"
+        if np.isfinite(want_loss):
+            assert abs(loss - want_loss) <= self.scale * bound.sum() + SHARE * abs(self.scale) * np.abs(want_row).sum(), "loss"
+        else:
+            assert loss == want_loss
+        if d is None:
+            return
+        # q + p: the absolute terms of the gradient
+        _, _, with_p = O.distill(self.z, self.ids, self.teacher, w, self.t, self.scale)
+        p = np.zeros(self.z.shape)
+        for r in range(rows):
+            for i, t in zip(self.ids[r], self.teacher[r]):
+                if 0 <= i < vocab and t > -np.inf:
+                    p[r, i] += np.exp((t - self.teacher[r][(self.ids[r] >= 0) & (self.ids[r] < vocab)].max()) / self.t)
+        p /= np.maximum(p.sum(1, keepdims=True), 1e-300)
+        size = np.abs(with_p) + 2 * abs(self.scale) * w[:, None] * self.t * p
+        bound = SHARE * m[:, None] * size + (0 if self.f32 else ULP) * np.abs(want_d) + 1e-37
+        assert np.isfinite(d).all()
+        off = np.abs(d - want_d)
+        assert (off <= bound).all(), f"dlogits: {np.max(off / bound):.3g} x the bound"
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab,k,pad", [(1, 1, 1, 0), (2, 7, 3, 0), (3, 8, 9, 1), (5, 1001, 1, 0), (4, 4096, 16, 8), (3, 8192, 64, 3),
+                                              (7, 8193, 5, 0), (2, 50021, 100, 0), (300, 777, 20, 0), (2, 131072, 7, 5),
+                                              (2, 140001, 1024, 2)])
+def test_sizes(rows, vocab, k, pad, f32):
+    Problem(rows, vocab, k, f32, pad=pad).check()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("temperature", [0.5, 2.0, 20.0])
+def test_temperatures(temperature, f32):
+    Problem(6, 3001, 12, f32, temperature).check()
+    Problem(3, 20000, 12, f32, temperature, weights=False).check()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab,pad,pad_out", [(1001, 0, 3), (9001, 7, 0), (9000, 0, 8), (40003, 1, 2)])
+def test_rows_that_start_anywhere(vocab, pad, pad_out, f32):
+    """Logits and gradient with leading dimensions of their own: rows start at every offset of 16 bytes."""
+    Problem(9, vocab, 10, f32, pad=pad, pad_out=pad_out).check()
+    Problem(9, vocab, 10, f32, pad=pad).check(in_place=True)
+    Problem(9, vocab, 10, f32, pad=pad).check(grad=False)
+    Problem(9, vocab, 10, f32, pad=pad, pad_out=pad_out).check(workspace=False)
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(12, 1003), (12, 30011), (400, 1003)])
+def test_rows_that_leave_nothing_and_masked_logits(rows, vocab, f32):
+    p = Problem(rows, vocab, 6, f32, seed=3)
+    low = -3.3895313892515355e38                          # the lowest bf16 value
+    p.w[0] = 0
+    p.z[0] = np.nan                                       # not looked at
+    p.ids[1] = -1
+    p.z[1, ::3] = np.inf
+    p.teacher[2] = -np.inf
+    p.z[3, :] = -np.inf                                   # no token is allowed
+    p.ids[4, 2], p.ids[4, 3], p.ids[4, 4] = vocab, -7, 2 ** 31 - 1   # padding
+    p.ids[5, 1] = p.ids[5, 0]                             # an id twice
+    p.teacher[6, 1:] = -np.inf
+    p.z[7, p.ids[7].max() + 1:] = -np.inf                 # masked
+    p.z[7, p.ids[7]] = 1.0
+    keep = p.ids[8]
+    p.z[8] = low
+    p.z[8, keep] = [1, 2, 3, -1, 0, 2]
+    p.z[9] = low                                          # the lowest value everywhere: uniform
+    p.teacher[10, 3] = -np.inf                            # a listed id that is masked on both sides
+    p.z[10, p.ids[10, 3]] = -np.inf
+    p.z[11] += 300.0 if f32 else 304.0
+    if not f32:
+        p.z[11] = bf16_round(p.z[11])
+    p.check()
+    p.check(in_place=True)
+    # the teacher wants what the student cannot give: an infinite loss, a finite gradient
+    p.z[5, p.ids[5, 3]] = -np.inf
+    row, loss, d = p.run()
+    assert row[5] == np.inf and loss == np.inf and np.isfinite(d).all()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+def test_one_id_is_the_cross_entropy(f32):
+    p = Problem(20, 5003, 1, f32, weights=False)
+    p.teacher[:] = -123.0
+    p.check()
+
+
+def test_large_listed_probabilities_meet_in_one_id():
+    """Every entry of a row names the same id."""
+    p = Problem(3, 2000, 33, True)
+    p.ids[:] = 17
+    p.check()
+
+
+def test_gradient_against_differences():
+    """In float32, along a direction: a central difference of width e has an error of e^2 / 6 of the third derivative (at
+    most the direction's size cubed over T^2), and the losses' rounding over e."""
+    p = Problem(8, 600, 10, True, temperature=1.5, weights=True)
+    _, _, d = p.run()
+    rng = np.random.default_rng(1)
+    way = rng.standard_normal(p.z.shape).astype(np.float32)
+    base, e = p.z, np.float32(2.0 ** -5)
+    total = []
+    for sign in (1, -1):
+        p.z = base + sign * e * way
+        total.append(p.run()[0].astype(np.float64).sum() * p.scale)
+    p.z = base
+    m = np.abs(base).max() / 1.5 + np.log(600) + 10
+    bound = 2 * p.scale * p.w.sum() * (1.5 ** 2 * m * SHARE / e + e ** 2 / 6 * np.abs(way).max() ** 3 / 1.5)
+    assert abs((total[0] - total[1]) / (2 * e) - (d.astype(np.float64) * way).sum()) <= bound
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 40000), (300, 9000)])
+def test_repeats_on_another_stream_and_in_a_graph(rows, vocab):
+    p = Problem(rows, vocab, 8, seed=9)
+    want = p.run()
+    st = rt.Stream()
+    got = p.run(stream=st.ptr)
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a, b)
+    z, dz = p._rows(p.z, p.ld), p._rows(np.zeros(p.z.shape), p.ldd)
+    ids, teacher, w = (rt.DeviceBuffer.from_numpy(a) for a in (p.ids, p.teacher, p.w))
+    row_loss, loss = rt.DeviceBuffer(4 * rows), rt.DeviceBuffer(4)
+    ws = rt.DeviceBuffer(rt.load().jpp_workspace_bytes(8, rows, 0, 0) + 16)
+    graph = rt.Graph(st)
+    with graph:
+        rt.distill_loss(z.ptr, ids.ptr, teacher.ptr, rows, vocab, 8, p.ld, row_loss.ptr, loss=loss.ptr, dlogits=dz.ptr,
+                        ldd=p.ldd, weight=w.ptr, temperature=p.t, scale=p.scale, workspace=ws.ptr, stream=st.ptr)
+    for _ in range(3):
+        graph.launch()
+        st.sync()
+        np.testing.assert_array_equal(row_loss.download(np.float32, (rows,)), want[0])
+        assert float(loss.download(np.float32, (1,))[0]) == want[1]
+        np.testing.assert_array_equal(rt.from_bf16_bits(dz.download(np.uint16, (rows, p.ldd)))[:, :vocab], want[2])
+        for b in (row_loss, loss, dz, ws):
+            b.zero()
+        rt.sync()

@@ -1,0 +1,313 @@
+"""Linear attention with a decay for each head on the GPU, against the float64 restatement.
+
+The tolerance follows from where the kernels round.  With A the same result of absolute values (every product
+and every sum positive):
+* bf16 results: their own rounding, half a unit in the last place, at most 2^-8 of the value (a full unit is
+  granted, for values on the edge); pairs and states enter the products as two bf16, 2^-16 of A, and f32 sums
+  of some hundred terms stay within another 2^-16: 2^-15 A.
+* f32 results (f32 tensors, and states of either type): f32 products and sums, 2^-18 A (64 roundings in the
+  same direction; thousands at random).
+"""
+import numpy as np
+import pytest
+
+from jaxpp_amd import runtime as rt
+from oracle import student as O
+from oracle.layers import bf16_round
+
+pytestmark = pytest.mark.gpu
+
+F32_SHARE, BF16_SHARE, BF16_ULP = 2.0 ** -18, 2.0 ** -15, 2.0 ** -8
+
+
+def _close(got, want, scale, f32, what):
+    got = got.astype(np.float64)
+    assert np.isfinite(got).all(), f"{what}: not finite"
+    bound = (F32_SHARE * scale if f32 else BF16_SHARE * scale + BF16_ULP * np.abs(want)) + 1e-30
+    worst = np.max(np.abs(got - want) / bound) if want.size else 0.0
+    assert worst <= 1, f"{what}: {worst:.3g} x the bound"
+
+
+class Tensor:
+    """[b, t, heads, d] on the device, each row with `pad` elements before and behind the heads, filled with NaN."""
+
+    def __init__(self, a, f32, pad):
+        self.shape, self.f32, self.pad = a.shape, f32, pad
+        b, t, h, d = a.shape
+        self.ld = h * d + 2 * pad
+        full = np.full((b * t, self.ld), np.nan, np.float32)
+        full[:, pad:pad + h * d] = a.reshape(b * t, h * d)
+        self.buf = rt.DeviceBuffer.from_numpy(full) if f32 else rt.DeviceBuffer.from_numpy(rt.to_bf16_bits(full))
+        self.ptr = self.buf.ptr + pad * (4 if f32 else 2)
+
+    def get(self):
+        b, t, h, d = self.shape
+        full = self.buf.download(np.float32 if self.f32 else np.uint16, (b * t, self.ld))
+        edge = full if self.f32 else rt.from_bf16_bits(full)
+        assert np.isnan(edge[:, :self.pad]).all() and np.isnan(edge[:, self.ld - self.pad:]).all(), "wrote beside its columns"
+        return edge[:, self.pad:self.ld - self.pad].reshape(self.shape)
+
+
+def _up(a):
+    return None if a is None else rt.DeviceBuffer.from_numpy(np.asarray(a, np.float32))
+
+
+def _ptr(b):
+    return None if b is None else b.ptr
+
+
+class Problem:
+    def __init__(self, batch, seq, heads, kv, dim, f32=False, lens=None, states=True, pad=8, seed=0, decay=None):
+        rng = np.random.default_rng(seed + 1000 * seq + heads)
+        r = lambda *s: rng.standard_normal(s).astype(np.float32) if f32 else bf16_round(rng.standard_normal(s).astype(np.float32))
+        self.sizes = dict(batch=batch, seq=seq, n_heads=heads, n_kv_heads=kv, head_dim=dim, scale=dim ** -0.5, f32=f32)
+        self.f32, self.lens, self.pad, self.rng = f32, lens, pad, rng
+        self.q, self.k, self.v, self.d_o = r(batch, seq, heads, dim), r(batch, seq, kv, dim), r(batch, seq, kv, dim), r(batch, seq, heads, dim)
+        spread = np.log1p(-2.0 ** -(1.0 + 8 * np.arange(heads) / max(heads - 1, 1)))
+        self.decay = (spread if decay is None else np.resize(decay, heads)).astype(np.float32)
+        shape = (batch, heads, dim, dim)
+        self.state = 3 * rng.standard_normal(shape).astype(np.float32) if states else None
+        self.d_state = rng.standard_normal(shape).astype(np.float32) if states else None
+
+    def _poisoned(self, a):
+        """The rows behind the sequences' ends hold what must not be read."""
+        if self.lens is None:
+            return a
+        a = a.copy()
+        for ib, n in enumerate(self.lens):
+            a[ib, max(n, 0):] = np.nan
+        return a
+
+    def _common(self, backward):
+        dev = {n: Tensor(self._poisoned(getattr(self, n)), self.f32, self.pad) for n in ("q", "k", "v", "d_o")}
+        dev["decay"] = _up(self.decay)
+        dev["lens"] = None if self.lens is None else rt.DeviceBuffer.from_numpy(np.asarray(self.lens, np.int32))
+        s = self.sizes
+        need = rt.linattn_workspace(s["batch"], s["seq"], s["n_heads"], s["n_kv_heads"], s["head_dim"], backward, self.f32)
+        dev["workspace"] = rt.DeviceBuffer.from_numpy(np.full(need // 4 + 16, np.nan, np.float32))
+        dev["need"] = need
+        return dev
+
+    def _guard(self, dev):
+        tail = dev["workspace"].download(np.float32, (16,), dev["need"])
+        assert np.isnan(tail).all(), "wrote behind the workspace"
+
+    def forward(self, in_place=True, stream=None):
+        dev = self._common(False)
+        o = Tensor(np.full(self.q.shape, 7.0), self.f32, self.pad)
+        state = _up(self.state)
+        out = None if state is None else state if in_place else rt.DeviceBuffer(state.nbytes)
+        rt.linattn_fwd(dev["q"].ptr, dev["k"].ptr, dev["v"].ptr, o.ptr, dev["decay"].ptr, dev["q"].ld, dev["k"].ld,
+                       dev["v"].ld, o.ld, state_in=_ptr(state), state_out=_ptr(out), lens=_ptr(dev["lens"]),
+                       workspace=dev["workspace"].ptr, stream=stream, **self.sizes)
+        rt.sync()
+        self._guard(dev)
+        return o.get(), None if out is None else out.download(np.float32, self.state.shape)
+
+    def check_forward(self, **kw):
+        o, s = self.forward(**kw)
+        args = (self.decay, self.sizes["scale"])
+        want, last = O.linattn(self.q, self.k, self.v, *args, self.state, self.lens)
+        mag, mag_last = O.linattn(*(np.abs(a) for a in (self.q, self.k, self.v)), *args,
+                                  None if self.state is None else np.abs(self.state), self.lens)
+        _close(o, want, mag, self.f32, "o")
+        if s is not None:
+            _close(s, last, mag_last, True, "state")
+
+    def backward(self):
+        dev = self._common(True)
+        dq, dk, dv = (Tensor(np.full(a.shape, 7.0), self.f32, self.pad) for a in (self.q, self.k, self.v))
+        state, d_state = _up(self.state), _up(self.d_state)
+        out = None if state is None else rt.DeviceBuffer(state.nbytes)
+        rt.linattn_bwd(dev["q"].ptr, dev["k"].ptr, dev["v"].ptr, dev["d_o"].ptr, dq.ptr, dk.ptr, dv.ptr,
+                       dev["decay"].ptr, dev["q"].ld, dev["k"].ld, dev["v"].ld, dev["d_o"].ld, dq.ld, dk.ld, dv.ld,
+                       state_in=_ptr(state), d_state_out=_ptr(d_state), d_state_in=_ptr(out), lens=_ptr(dev["lens"]),
+                       workspace=dev["workspace"].ptr, **self.sizes)
+        rt.sync()
+        self._guard(dev)
+        return dq.get(), dk.get(), dv.get(), None if out is None else out.download(np.float32, self.state.shape)
+
+    def check_backward(self):
+        got = self.backward()
+        args = (self.decay, self.sizes["scale"])
+        want = O.linattn_bwd(self.q, self.k, self.v, self.d_o, *args, self.state, self.d_state, self.lens)
+        mag = O.linattn_bwd(*(np.abs(a) for a in (self.q, self.k, self.v, self.d_o)), *args,
+                            None if self.state is None else np.abs(self.state),
+                            None if self.d_state is None else np.abs(self.d_state), self.lens)
+        for name, g, w, m in zip(("dq", "dk", "dv", "d_state"), got, want, mag):
+            if g is not None:
+                _close(g, w, m, self.f32 or name == "d_state", name)
+
+
+# lengths around the chunks (32, 64 rows) and the segments (128 rows and more) and their cuts
+SIZES = [(1, 1, 1, 1, 64), (2, 2, 2, 2, 128), (1, 31, 2, 1, 64), (1, 33, 1, 1, 128), (2, 63, 4, 2, 64), (1, 64, 3, 3, 128),
+         (3, 65, 2, 1, 64), (1, 127, 6, 2, 128), (1, 130, 4, 4, 64), (1, 257, 2, 2, 128), (2, 300, 8, 1, 64),
+         (1, 520, 4, 2, 128), (1, 1100, 2, 2, 64)]
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("batch,seq,heads,kv,dim", SIZES)
+def test_forward(batch, seq, heads, kv, dim, f32):
+    Problem(batch, seq, heads, kv, dim, f32).check_forward()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("batch,seq,heads,kv,dim", SIZES)
+def test_backward(batch, seq, heads, kv, dim, f32):
+    Problem(batch, seq, heads, kv, dim, f32, seed=1).check_backward()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("seq,lens", [(70, [70, 0, 1, 64]), (300, [299, 128, 0, 65]), (400, [500, -3, 129, 400])])
+def test_sequences_of_different_lengths(seq, lens, dim, f32):
+    """Rows behind the ends hold NaN; lengths beyond the range are held to it."""
+    held = [min(max(n, 0), seq) for n in lens]
+    for states in (True, False):
+        p = Problem(4, seq, 2, 1, dim, f32, held, states, seed=2)
+        p.check_forward(in_place=False)
+        p.check_backward()
+    p.lens = lens
+    a = p.forward()
+    p.lens = held
+    np.testing.assert_array_equal(a[0], p.forward()[0])
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("seq", [64, 300])
+def test_decays_at_the_ends_of_their_range(seq, f32):
+    """No memory (log 0), next to none, none lost, and a factor of 0.999."""
+    p = Problem(1, seq, 6, 6, 64, f32, decay=[-np.inf, -200.0, -90.0, -3.0, -1e-3, 0.0])
+    p.check_forward()
+    p.check_backward()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+def test_no_states_and_many_walks(f32):
+    """Enough heads that a sequence is one workgroup's, without states."""
+    p = Problem(8, 300, 64, 64, 64, f32, states=False, pad=0)
+    p.check_forward()
+    p.check_backward()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+def test_no_rows_hand_the_state_on(f32):
+    p = Problem(2, 0, 2, 1, 64, f32, pad=0)
+    _, s = p.forward(in_place=False)
+    np.testing.assert_array_equal(s, p.state)
+    np.testing.assert_array_equal(p.backward()[3], p.d_state)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_prompt_in_two_parts_and_token_by_token(dim):
+    """The state carries a prompt over calls of the forward, and over single tokens, into the same result."""
+    p = Problem(2, 150, 4, 2, dim, f32=True, pad=0)
+    whole, last = p.forward()
+    parts = []
+    state = p.state
+    for a, b in ((0, 97), (97, 147)):
+        part = Problem(2, b - a, 4, 2, dim, f32=True, pad=0)
+        part.q, part.k, part.v, part.state = p.q[:, a:b], p.k[:, a:b], p.v[:, a:b], state
+        o, state = part.forward()
+        parts.append(o)
+    dev = _up(state)
+    decay = _up(p.decay)
+    for t in range(147, 150):
+        q, k, v = (Tensor(x[:, t:t + 1], True, 4) for x in (p.q, p.k, p.v))
+        o = Tensor(np.zeros((2, 1, 4, dim)), True, 8)
+        sizes = {n: x for n, x in p.sizes.items() if n != "seq"}
+        rt.linattn_step(q.ptr, k.ptr, v.ptr, o.ptr, decay.ptr, dev.ptr, dev.ptr, q.ld, k.ld, v.ld, o.ld, **sizes)
+        rt.sync()
+        parts.append(o.get())
+    args = (p.decay, p.sizes["scale"])
+    want, want_last = O.linattn(p.q, p.k, p.v, *args, p.state)
+    mag, mag_last = O.linattn(*(np.abs(a) for a in (p.q, p.k, p.v)), *args, np.abs(p.state))
+    _close(np.concatenate(parts, 1), want, mag, True, "o in parts")
+    _close(whole, want, mag, True, "o at once")
+    _close(dev.download(np.float32, p.state.shape), want_last, mag_last, True, "state in parts")
+    _close(last, want_last, mag_last, True, "state at once")
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("batch,heads,kv,dim", [(1, 1, 1, 64), (3, 4, 2, 128), (5, 7, 1, 64), (70, 8, 8, 128)])
+@pytest.mark.parametrize("states", [False, True])
+def test_step(batch, heads, kv, dim, f32, states):
+    p = Problem(batch, 1, heads, kv, dim, f32, seed=4)
+    p.decay[0] = -np.inf
+    q, k, v = (Tensor(a, f32, 8) for a in (p.q, p.k, p.v))
+    o, decay = Tensor(np.zeros(p.q.shape), f32, 8), _up(p.decay)
+    state = _up(p.state) if states else None
+    out = rt.DeviceBuffer(p.state.nbytes)
+    sizes = {n: x for n, x in p.sizes.items() if n != "seq"}
+    rt.linattn_step(q.ptr, k.ptr, v.ptr, o.ptr, decay.ptr, _ptr(state), out.ptr, q.ld, k.ld, v.ld, o.ld, **sizes)
+    rt.sync()
+    s0 = p.state if states else None
+    want, last = O.linattn_recurrence(p.q, p.k, p.v, p.decay, p.sizes["scale"], s0)
+    mag, mag_last = O.linattn_recurrence(*(np.abs(a) for a in (p.q, p.k, p.v)), p.decay, p.sizes["scale"],
+                                         None if s0 is None else np.abs(s0))
+    _close(o.get(), want, mag, f32, "o")
+    _close(out.download(np.float32, p.state.shape), last, mag_last, True, "state")
+
+
+def test_gradients_against_differences_of_the_forward():
+    """The output is linear in each operand, so a central difference of width 1 is exact but for rounding: with N
+    terms of size at most m in the sum over the output, 2^-18 of their absolute sum."""
+    p = Problem(2, 200, 2, 2, 64, f32=True, states=True, pad=0, seed=6)
+    grads = dict(zip(("q", "k", "v", "state"), p.backward()))
+    rng = np.random.default_rng(1)
+    for name, grad in grads.items():
+        base, way = getattr(p, name), rng.standard_normal(getattr(p, name).shape).astype(np.float32)
+        sums = []
+        size = 0.0
+        for sign in (1, -1):
+            setattr(p, name, base + np.float32(sign) * way)
+            o, s = p.forward()
+            terms = [o.astype(np.float64) * p.d_o, s.astype(np.float64) * p.d_state]
+            sums.append(sum(t.sum() for t in terms))
+            mag = O.linattn(np.abs(p.q), np.abs(p.k), np.abs(p.v), p.decay, p.sizes["scale"], np.abs(p.state))
+            size += (mag[0] * np.abs(p.d_o)).sum() + (mag[1] * np.abs(p.d_state)).sum()
+        setattr(p, name, base)
+        want = (grad.astype(np.float64) * way).sum()
+        assert abs((sums[0] - sums[1]) / 2 - want) <= F32_SHARE * size, name
+
+
+def test_another_stream_repeats_and_graphs():
+    """On a stream of its own, recorded and replayed with other work between: the same bits."""
+    p = Problem(1, 700, 4, 2, 128, pad=0, seed=8)
+    want_o, want_s = p.forward(in_place=False)
+    want_g = p.backward()
+    st = rt.Stream()
+    dev = p._common(True)
+    o = Tensor(np.zeros(p.q.shape), False, 0)
+    grads = [Tensor(np.zeros(a.shape), False, 0) for a in (p.q, p.k, p.v)]
+    state, d_state = _up(p.state), _up(p.d_state)
+    out, d_out = rt.DeviceBuffer(state.nbytes), rt.DeviceBuffer(state.nbytes)
+
+    def calls():
+        ld = [dev[n].ld for n in "qkv"]
+        rt.linattn_fwd(dev["q"].ptr, dev["k"].ptr, dev["v"].ptr, o.ptr, dev["decay"].ptr, *ld, o.ld,
+                       state_in=state.ptr, state_out=out.ptr, workspace=dev["workspace"].ptr, stream=st.ptr, **p.sizes)
+        rt.linattn_bwd(dev["q"].ptr, dev["k"].ptr, dev["v"].ptr, dev["d_o"].ptr, *(g.ptr for g in grads),
+                       dev["decay"].ptr, *ld, dev["d_o"].ld, *(g.ld for g in grads), state_in=state.ptr,
+                       d_state_out=d_state.ptr, d_state_in=d_out.ptr, workspace=dev["workspace"].ptr, stream=st.ptr,
+                       **p.sizes)
+
+    def check():
+        st.sync()
+        np.testing.assert_array_equal(o.get(), want_o)
+        np.testing.assert_array_equal(out.download(np.float32, p.state.shape), want_s)
+        for g, w in zip(grads, want_g):
+            np.testing.assert_array_equal(g.get(), w)
+        np.testing.assert_array_equal(d_out.download(np.float32, p.state.shape), want_g[3])
+        for buf in (o.buf, out, d_out, dev["workspace"], *(g.buf for g in grads)):
+            buf.zero()
+        rt.sync()
+
+    calls()
+    check()
+    graph = rt.Graph(st)
+    with graph:
+        calls()
+    for _ in range(3):
+        graph.launch()
+        check()

@@ -1,0 +1,109 @@
+"""The float64 restatements that the GPU tests of a linear-attention student's operators are held to:
+against each other and against differences (no GPU)."""
+import numpy as np
+import pytest
+
+from oracle import student as O
+
+
+def _lin(rng, b, t, h, hk, d, states=True):
+    r = rng.standard_normal
+    c = dict(q=r((b, t, h, d)), k=r((b, t, hk, d)), v=r((b, t, hk, d)),
+             decay=np.log1p(-1.0 / np.array([2.0 ** (1 + i % 5) for i in range(h)])))
+    c["state"] = r((b, h, d, d)) if states else None
+    return c
+
+
+@pytest.mark.parametrize("b,t,h,hk,d,lens", [(1, 1, 1, 1, 4, None), (2, 9, 4, 2, 8, [9, 4]), (3, 5, 3, 1, 4, [0, 1, 5])])
+@pytest.mark.parametrize("states", [False, True])
+def test_linear_attention_by_pairs_is_the_recurrence(b, t, h, hk, d, lens, states):
+    c = _lin(np.random.default_rng(b * 100 + t), b, t, h, hk, d, states)
+    c["decay"][0] = -np.inf                      # a head without memory
+    o, s = O.linattn(**c, scale=0.3, lens=lens)
+    o2, s2 = O.linattn_recurrence(**c, scale=0.3, lens=lens)
+    np.testing.assert_allclose(o, o2, rtol=1e-12, atol=1e-12)
+    np.testing.assert_allclose(s, s2, rtol=1e-12, atol=1e-12)
+
+
+def test_linear_attention_gradients_against_differences():
+    """The output is linear in each operand: a central difference of any width is exact."""
+    rng = np.random.default_rng(5)
+    c = _lin(rng, 2, 7, 4, 2, 4)
+    lens = [7, 3]
+    d_o, d_s = rng.standard_normal((2, 7, 4, 4)), rng.standard_normal((2, 4, 4, 4))
+
+    def value(**change):
+        o, s = O.linattn(**{**c, **change}, scale=0.7, lens=lens)
+        return (o * d_o).sum() + (s * d_s).sum()
+
+    grads = dict(zip(("q", "k", "v", "state"), O.linattn_bwd(**c, d_o=d_o, d_state=d_s, scale=0.7, lens=lens)))
+    for name, grad in grads.items():
+        for _ in range(8):
+            at = tuple(rng.integers(0, n) for n in c[name].shape)
+            step = np.zeros_like(c[name])
+            step[at] = 0.5
+            got = value(**{name: c[name] + step}) - value(**{name: c[name] - step})
+            assert abs(got - grad[at]) <= 1e-10 * (1 + abs(got)), (name, at)
+
+
+@pytest.mark.parametrize("post,gate_rows,pre", [(True, 6, True), (True, 2, True), (False, 3, True), (True, 0, False),
+                                                (False, 6, False), (False, 0, True)])
+def test_block_join_gradients_against_differences(post, gate_rows, pre):
+    rng = np.random.default_rng(11)
+    rows, cols, alpha, eps = 6, 5, 0.8, 1e-3
+    r = rng.standard_normal
+    c = dict(x=r((rows, cols)), b=r((rows, cols)), gamma_post=1 + 0.2 * r(cols) if post else None,
+             gate=r((rows // gate_rows, cols)) if gate_rows else None, gamma_pre=1 + 0.2 * r(cols) if pre else None)
+    dh, dy = r((rows, cols)), r((rows, cols))
+
+    def value(**change):
+        o = O.block_join(**{**c, **change}, gate_rows=gate_rows, alpha=alpha, eps=eps)
+        return (o["h"] * dh).sum() + ((o["y"] * dy).sum() if pre else 0.0)
+
+    o = O.block_join(**c, gate_rows=gate_rows, alpha=alpha, eps=eps)
+    g = O.block_join_bwd(o["h"], c["b"], dh, dy, c["gamma_post"], c["gate"], gate_rows, c["gamma_pre"],
+                         o.get("rstd_post"), o.get("rstd_pre"), alpha)
+    for name, grad in (("x", "dx"), ("b", "db"), ("gamma_post", "dgamma_post"), ("gate", "dgate"), ("gamma_pre", "dgamma_pre")):
+        if c[name] is None:
+            assert grad not in g
+            continue
+        for at in np.ndindex(*c[name].shape):
+            step = np.zeros_like(c[name])
+            step[at] = 1e-5
+            got = (value(**{name: c[name] + step}) - value(**{name: c[name] - step})) / 2e-5
+            assert abs(got - g[grad][at]) <= 1e-6 * (1 + abs(got)), (name, at)
+
+
+def test_distillation_gradient_against_differences():
+    rng = np.random.default_rng(3)
+    rows, vocab, k = 6, 11, 4
+    z, teacher = rng.standard_normal((rows, vocab)), rng.standard_normal((rows, k))
+    ids = np.stack([rng.permutation(vocab)[:k] for _ in range(rows)])
+    ids[1] = -1                                   # nothing listed
+    ids[2, 0], ids[2, 1] = vocab, ids[2, 2]       # padding, and an id twice
+    teacher[3, :2] = -np.inf
+    w = np.array([1, 1, 0.5, 2, 0, 1.0])
+    z[5, 3] = -np.inf
+    ids[5] = [0, 1, 2, 4]
+    loss, grad = (lambda f: (f[1], f[2]))(O.distill(z, ids, teacher, w, 1.7, 0.4))
+    assert np.isfinite(loss) and not grad[1].any() and not grad[4].any()
+    for r in range(rows):
+        for c in range(vocab):
+            if z[r, c] == -np.inf:
+                assert grad[r, c] == 0
+                continue
+            step = np.zeros_like(z)
+            step[r, c] = 1e-5
+            got = (O.distill(z + step, ids, teacher, w, 1.7, 0.4)[1] - O.distill(z - step, ids, teacher, w, 1.7, 0.4)[1]) / 2e-5
+            assert abs(got - grad[r, c]) <= 1e-8, (r, c)
+
+
+def test_distillation_of_one_id_is_the_cross_entropy():
+    rng = np.random.default_rng(4)
+    z = rng.standard_normal((3, 7))
+    ids = np.array([[2], [0], [6]])
+    row, loss, grad = O.distill(z, ids, np.zeros((3, 1)))
+    log_q = z - np.log(np.exp(z).sum(1, keepdims=True))
+    np.testing.assert_allclose(row, -log_q[np.arange(3), ids[:, 0]], rtol=1e-12)
+    np.testing.assert_allclose(grad.sum(1), 0, atol=1e-12)
+    assert abs(loss - row.sum()) <= 1e-12

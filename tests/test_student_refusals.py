@@ -1,0 +1,148 @@
+"""What the operators of a linear-attention student refuse, on the host and before any launch (no GPU)."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from jaxpp_amd import runtime as rt
+
+AT = 1 << 20          # an address that is never looked at
+
+
+def _refused(fn, args, match, *more):
+    assert getattr(rt.load(), fn)(*more, C.byref(args)) == -1, fn
+    assert match in rt.load().jpp_last_error().decode(), rt.load().jpp_last_error()
+
+
+def _lin(**change):
+    a = dict(q=AT, k=2 * AT, v=3 * AT, o=4 * AT, d_o=5 * AT, dq=6 * AT, dk=7 * AT, dv=8 * AT, decay=AT, workspace=9 * AT,
+             ldq=256, ldk=128, ldv=128, ldo=256, lddo=256, lddq=256, lddk=128, lddv=128, batch=2, seq=300, n_heads=4,
+             n_kv_heads=2, head_dim=64, scale=1.0, dtype=0)
+    a.update(change)
+    return rt.LinattnArgs(**a)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(dtype=2), "dtype"), (dict(batch=-1), "batch"), (dict(seq=-1), "seq"), (dict(head_dim=96), "head_dim"),
+    (dict(n_kv_heads=3), "heads"), (dict(n_heads=0), "heads"), (dict(q=None), "q"), (dict(v=3 * AT + 8), "alignment"),
+    (dict(ldk=120), "leading dimension of k"), (dict(ldq=260), "alignment"), (dict(decay=None), "decay"),
+    (dict(batch=1 << 21), "too many")])
+def test_linear_attention(change, match):
+    for fn in ("jpp_linattn_fwd", "jpp_linattn_bwd", "jpp_linattn_step"):
+        if fn == "jpp_linattn_step":
+            change = {**change, "state_out": AT}
+            if "seq" in change:
+                continue
+        _refused(fn, _lin(**change), match if match != "decay" or fn != "jpp_linattn_step" else "null", None)
+
+
+def test_linear_attention_operands_of_each_direction():
+    _refused("jpp_linattn_fwd", _lin(o=None), "o", None)
+    _refused("jpp_linattn_fwd", _lin(o=3 * AT), "overlaps", None)
+    _refused("jpp_linattn_fwd", _lin(workspace=None), "workspace", None)
+    _refused("jpp_linattn_fwd", _lin(state_in=AT + 4), "state_in", None)
+    _refused("jpp_linattn_fwd", _lin(dtype=1, ldo=258), "alignment", None)
+    _refused("jpp_linattn_bwd", _lin(d_o=None), "d_o", None)
+    _refused("jpp_linattn_bwd", _lin(dk=5 * AT), "overlaps", None)
+    _refused("jpp_linattn_bwd", _lin(dk=6 * AT), "overlap", None)
+    _refused("jpp_linattn_bwd", _lin(lddv=64), "leading dimension of dv", None)
+    _refused("jpp_linattn_bwd", _lin(d_state_out=AT * 11, d_state_in=AT * 11), "d_state_in", None)
+    _refused("jpp_linattn_step", _lin(), "null", None)
+    assert rt.load().jpp_linattn_fwd(None, None) == -1
+    # nothing to do
+    assert rt.load().jpp_linattn_fwd(None, C.byref(_lin(batch=0, q=None))) == 0
+    assert rt.load().jpp_linattn_step(None, C.byref(_lin(batch=0))) == 0
+
+
+def test_linear_attention_workspace():
+    assert rt.linattn_workspace(1, 64, 4, 4, 64) == 0                    # one segment
+    assert rt.linattn_workspace(64, 4096, 32, 32, 128) == 0              # heads enough without segments
+    one = rt.linattn_workspace(1, 4096, 4, 4, 128)
+    assert one > 0 and one % (4 * 4 * 128 * 128) == 0
+    shared = rt.linattn_workspace(1, 4096, 4, 2, 128, backward=True)
+    assert shared - rt.linattn_workspace(1, 4096, 4, 4, 128, backward=True) == 2 * 4 * 4096 * 4 * 128
+    assert rt.linattn_workspace(1, 4096, 4, 3, 128) == 0 and rt.linattn_workspace(1, 0, 4, 4, 64) == 0
+
+
+def _join(**change):
+    a = dict(x=AT, b=2 * AT, gamma_post=3 * AT, gate=4 * AT, gamma_pre=5 * AT, h=6 * AT, y=7 * AT, rstd_post=8 * AT,
+             rstd_pre=9 * AT, dh=10 * AT, dy=11 * AT, dx=12 * AT, db=13 * AT, dgamma_post=14 * AT, dgate=15 * AT,
+             dgamma_pre=16 * AT, workspace=17 * AT, rows=6, cols=512, gate_rows=3, alpha=1.0, eps=1e-6)
+    a.update(change)
+    return rt.JoinArgs(**a)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(dtype=7), "dtype"), (dict(cols=8200), "cols"), (dict(cols=12), "cols"), (dict(cols=0), "cols"), (dict(rows=-1), "rows"),
+    (dict(rows=1 << 40), "too many"), (dict(b=None), "null"), (dict(gate_rows=4), "gate rows"), (dict(gate_rows=0), "gate rows"),
+    (dict(rstd_post=None), "rstd_post"), (dict(rstd_pre=None), "rstd_pre"), (dict(gamma_pre=5 * AT + 2), "alignment"),
+    (dict(h=None), "null")])
+def test_block_join(change, match):
+    _refused("jpp_block_join_fwd", _join(**change), match, None)
+    _refused("jpp_block_join_bwd", _join(**change), match, None)
+
+
+def test_block_join_operands_of_each_direction():
+    _refused("jpp_block_join_fwd", _join(x=None), "null", None)
+    _refused("jpp_block_join_fwd", _join(y=None), "null", None)
+    _refused("jpp_block_join_fwd", _join(y=6 * AT), "overlaps", None)
+    _refused("jpp_block_join_bwd", _join(dy=None), "null", None)
+    _refused("jpp_block_join_bwd", _join(gamma_pre=None, dgamma_pre=None, dh=None), "cotangent", None)
+    _refused("jpp_block_join_bwd", _join(gamma_pre=None), "dgamma_pre", None)
+    _refused("jpp_block_join_bwd", _join(gamma_post=None), "dgamma_post", None)
+    _refused("jpp_block_join_bwd", _join(gate=None), "dgate", None)
+    _refused("jpp_block_join_bwd", _join(workspace=None), "workspace", None)
+    _refused("jpp_block_join_bwd", _join(db=12 * AT), "overlap", None)
+    _refused("jpp_block_join_bwd", _join(db=10 * AT), "overlap", None)
+    assert rt.load().jpp_block_join_fwd(None, None) == -1
+    assert rt.load().jpp_block_join_fwd(None, C.byref(_join(rows=0, x=None))) == 0
+    assert rt.load().jpp_workspace_bytes(7, 512, 3, 0) == 2 * (3 + 512) * 512 * 4
+
+
+def _distill(**change):
+    a = dict(logits=AT, ids=2 * AT, teacher=3 * AT, row_loss=4 * AT, loss=5 * AT, dlogits=6 * AT, ld=1000, ldd=1000, rows=4,
+             vocab=1000, k=8, temperature=1.0, scale=1.0)
+    a.update(change)
+    return rt.DistillArgs(**a)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(dtype=3), "dtype"), (dict(rows=-1), "logits"), (dict(vocab=0), "logits"), (dict(rows=1 << 40), "logits"),
+    (dict(k=0), "k 0"), (dict(k=1025), "k 1025"), (dict(temperature=0.0), "temperature"),
+    (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"), (dict(temperature=1e-40), "temperature"),
+    (dict(logits=None), "null"), (dict(ids=None), "null"), (dict(teacher=None), "null"), (dict(row_loss=None), "null"),
+    (dict(ld=999), "leading"), (dict(ldd=999), "leading"), (dict(logits=AT + 2), "aligned"), (dict(dlogits=AT + 8), "aligned"),
+    (dict(dlogits=AT, ldd=1008), "over logits")])
+def test_distillation(change, match):
+    _refused("jpp_distill_loss", _distill(**change), match, None)
+
+
+def test_distillation_of_nothing():
+    assert rt.load().jpp_distill_loss(None, None) == -1
+    assert rt.load().jpp_distill_loss(None, C.byref(_distill(rows=0, loss=None, logits=None))) == 0
+    assert rt.load().jpp_workspace_bytes(8, 5, 0, 0) == 5 * 64 * 8 and rt.load().jpp_workspace_bytes(8, 4096, 0, 0) == 0
+
+
+def test_structs_match_the_header_as_a_c_compiler_sees_it(tmp_path):
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    pairs = {"jpp_linattn_args": rt.LinattnArgs, "jpp_join_args": rt.JoinArgs, "jpp_distill_args": rt.DistillArgs}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "jaxpp_amd.h"', 'int main(void) {']
+    for cname, cls in pairs.items():
+        lines.append(f'  printf("{cname} %zu\\n", sizeof({cname}));')
+        lines += [f'  printf("{cname}.{f} %zu\\n", offsetof({cname}, {f}));' for f, _ in cls._fields_]
+    lines += ['  printf("ws %d %d\\n", JPP_WS_BLOCK_JOIN, JPP_WS_DISTILL);', '  return 0;', '}']
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines))
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run([cc, "-std=c99", "-I", include, str(src), "-o", str(exe)], check=True, capture_output=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+    assert out.pop() == "ws 7 8"
+    got = dict(line.split() for line in out)
+    for cname, cls in pairs.items():
+        assert int(got[cname]) == C.sizeof(cls), cname
+        for f, _ in cls._fields_:
+            assert int(got[f"{cname}.{f}"]) == getattr(cls, f).offset, f"{cname}.{f}"
