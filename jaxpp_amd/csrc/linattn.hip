@@ -26,9 +26,7 @@
 
 #include "attention_common.h"
 
-using jpp_attn::acc_to_frag;
 using jpp_attn::pack2;
-using jpp_attn::slabs_frag;
 
 namespace {
 
@@ -44,6 +42,7 @@ struct Role {
   int gx, gy, gz, go;            // query heads per head of each tensor
   int reverse;                   // walk from the last row to the first
   int init_transposed;           // `init` holds the state's transpose
+  int parts_transposed;          // and so does `parts`, another role's
   int out_f32;
   float a_pair, a_state, a_update;  // factors of the pair sum, of the state's part and of y^T z in the state
   const float* init;             // [batch, heads, D, D] or null (zero)
@@ -53,7 +52,7 @@ struct Role {
 
 struct Params {
   Role role[kMaxRoles];
-  int n_roles;
+  int n_roles, n_sums;           // of which the first n_sums own their `parts`
   const float* decay;
   const int32_t* lens;
   int batch, seq, heads, n_seg, seg_rows;
@@ -80,11 +79,11 @@ __device__ __forceinline__ int rows_of(const Params& p, int b) {
 
 // Workgroups of one (segment, batch) follow each other over the heads, and the roles over those: what
 // they share is read at about the same time.
-__device__ __forceinline__ Place place(const Params& p) {
+__device__ __forceinline__ Place place(const Params& p, int n_roles) {
   Place w;
   unsigned i = blockIdx.x;
-  w.role = i % p.n_roles;
-  i /= p.n_roles;
+  w.role = i % n_roles;
+  i /= n_roles;
   w.h = i % p.heads;
   i /= p.heads;
   w.seg = i % p.n_seg;
@@ -98,16 +97,38 @@ __device__ __forceinline__ Place place(const Params& p) {
 
 __device__ __forceinline__ float decay_pow(float g2, int n) { return exp2f(g2 * (float)n); }
 
-// 8 floats -> the bf16 operand nearest to them, and what that leaves
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ bf16x8 split(f32x8& v) {
-  const bf16x8 hi = __builtin_convertvector(v, bf16x8);
-  v -= __builtin_convertvector(hi, f32x8);
-  return hi;
+// Eight floats as the MFMA operand nearest to them (two elements per conversion), and, in place, what that leaves.
+__device__ __forceinline__ bf16x8 split(float (&v)[8]) {
+  uint4 w;
+  uint32_t* const u = (uint32_t*)&w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u[i] = pack2(v[2 * i], v[2 * i + 1]);
+    v[2 * i] -= bf16lo_to_f32(u[i]);
+    v[2 * i + 1] -= bf16hi_to_f32(u[i]);
+  }
+  return __builtin_bit_cast(bf16x8, w);
 }
-__device__ __forceinline__ f32x8 acc8(const f32x16& a, int base) {
-  return f32x8{a[base], a[base + 1], a[base + 2], a[base + 3], a[base + 4], a[base + 5], a[base + 6], a[base + 7]};
+__device__ __forceinline__ bf16x8 nearest(const float (&v)[8]) {
+  return __builtin_bit_cast(bf16x8, make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])));
 }
+__device__ __forceinline__ void acc8(float (&v)[8], const f32x16& a, int base) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = a[base + e];
+}
+__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// LDS by byte addresses, so that tiles, slabs and row blocks are offsets of the instruction
+template <class V> __device__ __forceinline__ V lds_get(uint32_t at) {
+  return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
+}
+template <class V> __device__ __forceinline__ void lds_put(uint32_t at, const V& v) {
+  *(__attribute__((address_space(3))) V*)(uintptr_t)at = v;
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
 // bf16 tiles: [64][D] in LDS as D / 64 swizzled slabs, staged through registers (rows behind
@@ -119,52 +140,95 @@ struct Tile {
   static constexpr int BYTES = kChunk * D * 2;
   static constexpr int UNITS = D / 8;                // 16-byte units of a row
   static constexpr int PER = kChunk * UNITS / THREADS;
-  static_assert(PER == 4, "four units per thread");
+  static_assert(PER == 4 && THREADS / UNITS == 16, "a thread has a unit of every 16th row");
+  typedef u32x4 Regs[PER];
 
-  static __device__ __forceinline__ void load(uint4 (&r)[PER], const bf16_t* src, long ld, int live) {
+  // the thread's byte offset from a chunk's first row, and its place in a tile (rows 16 apart have the
+  // same swizzle)
+  static __device__ __forceinline__ uint32_t offset(long ld) {
+    return (uint32_t)((threadIdx.x / UNITS) * ld + (threadIdx.x % UNITS) * 8) * 2;
+  }
+  static __device__ __forceinline__ uint32_t unit() {
+    const int c = threadIdx.x % UNITS;
+    return (c >> 3) * 8192 + slab_off(threadIdx.x / UNITS, c & 7);
+  }
+  static __device__ __forceinline__ void load(Regs& r, const bf16_t* src, long ld, uint32_t off, int live) {
+    const uint8_t* base = (const uint8_t*)src;
+    if (live >= kChunk) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
-      r[i] = row < live ? *(const uint4*)(src + row * ld + c * 8) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < PER; ++i) r[i] = *(const u32x4*)(base + 32 * i * ld + off);
+    } else {
+      const int row = threadIdx.x / UNITS;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        r[i] = row + 16 * i < live ? *(const u32x4*)(base + 32 * i * ld + off) : u32x4{0, 0, 0, 0};
     }
   }
-  static __device__ __forceinline__ uint8_t* unit(uint8_t* tile, int i) {
-    const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
-    return tile + (c >> 3) * 8192 + slab_off(row, c & 7);
-  }
-  static __device__ __forceinline__ void put(uint8_t* tile, const uint4 (&r)[PER]) {
+  static __device__ __forceinline__ void put(uint32_t at, const Regs& r) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) *(uint4*)unit(tile, i) = r[i];
+    for (int i = 0; i < PER; ++i) lds_put(at + i * 2048, r[i]);
   }
 };
 
-// z of one chunk as MFMA operand (contraction over the rows, in the accumulators' order), times
-// the rows' weights, in three parts that together hold all 24 bits of the products: the state
-// is an f32 result, and its terms are as exact as f32 products.
-template <int D>
-__device__ __forceinline__ void update_state(f32x16 (&S)[D / 32], const uint8_t* ytile, const bf16x8 (&zf)[4],
-                                             float g2, float a_update, int rows, bool reverse, int lane) {
-  const float keep = decay_pow(g2, rows);
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t) S[t] *= keep;
+// Operand whose rows are a tile's columns 32 t .. + 31 and whose contraction runs over the tile's rows 16 st .. + 15 in the
+// accumulators' order (as slab_frag_tr): `at` = the tile's address + tr_base(lane).
+__device__ __forceinline__ uint32_t tr_base(int lane) {
+  const int g = lane >> 4, s = lane & 15;
+  const int k = ((g >> 1) << 2) + (s >> 2), n = ((g & 1) << 4) + ((s & 3) << 2);
+  return slab_off(k, n >> 3) + ((n & 7) << 1);
+}
+__device__ __forceinline__ bf16x8 tr_frag(uint32_t at, int t, int st) {
+  // 8 rows, like 32 columns, flip bit 2 of the 16-byte unit
+  const uint32_t even = at + (t >> 1) * 8192 + st * 2048, odd = (at ^ 64) + (t >> 1) * 8192 + st * 2048;
+  typedef __attribute__((address_space(3))) s16x4* p16;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)(t & 1 ? odd : even));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)((t & 1 ? even : odd) + 1024));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A head's decay by distances, in LDS: of pairs (i - j + 64, zero on the side that does not count), and of the
+// chunk's rows in the state's update and in what they take from it.
+struct Weights {
+  float pair[128], up[kChunk], state[kChunk];
+};
+__device__ __forceinline__ void pair_weights(Weights* w, float g2, float a_pair, bool rev) {
+  for (int k = threadIdx.x; k < 128; k += blockDim.x) {
+    const int far = rev ? 64 - k : k - 64;
+    w->pair[k] = far >= 0 ? a_pair * decay_pow(g2, far) : 0.f;
+  }
+}
+__device__ __forceinline__ void row_weights(Weights* w, float g2, float a_update, float a_state, int rows, bool rev) {
+  if (threadIdx.x < kChunk) {
+    const int j = threadIdx.x, from_end = max(rows - 1 - j, 0);   // (rows behind the end are zero)
+    w->up[j] = a_update * decay_pow(g2, rev ? j + 1 : from_end);
+    w->state[j] = a_state * decay_pow(g2, rev ? from_end : j + 1);
+  }
+}
+
+// S += y^T (w z): z as operand times its rows' weights in PARTS bf16 - three hold all 24 bits of the
+// products, for a state that is a result; two, 16 bits, for one that only meets x as two bf16.
+template <int D, int PARTS>
+__device__ __forceinline__ void update_state(f32x16 (&S)[D / 32], uint32_t ytr, const bf16x8 (&zf)[4], uint32_t up,
+                                             int lane) {
 #pragma unroll
   for (int st = 0; st < 4; ++st) {
-    f32x8 z = __builtin_convertvector(zf[st], f32x8);
+    const u32x4 zw = __builtin_bit_cast(u32x4, zf[st]);
+    const f32x4 w0 = lds_get<f32x4>(up + (lane >> 5) * 16 + st * 64);
+    const f32x4 w1 = lds_get<f32x4>(up + (lane >> 5) * 16 + st * 64 + 32);
+    float z[8] = {bf16lo_to_f32(zw.x) * w0.x, bf16hi_to_f32(zw.x) * w0.y, bf16lo_to_f32(zw.y) * w0.z,
+                  bf16hi_to_f32(zw.y) * w0.w, bf16lo_to_f32(zw.z) * w1.x, bf16hi_to_f32(zw.z) * w1.y,
+                  bf16lo_to_f32(zw.w) * w1.z, bf16hi_to_f32(zw.w) * w1.w};
+    bf16x8 part[PARTS];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = st * 16 + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3);
-      // (rows behind the end are zero, and their exponent is kept from going the other way)
-      z[e] *= a_update * decay_pow(g2, reverse ? j + 1 : max(rows - 1 - j, 0));
-    }
-    bf16x8 part[3];
+    for (int i = 0; i + 1 < PARTS; ++i) part[i] = split(z);
+    part[PARTS - 1] = nearest(z);
+    bf16x8 yf[D / 32];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) part[i] = split(z);
+    for (int t = 0; t < D / 32; ++t) yf[t] = tr_frag(ytr, t, st);
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t) {
-      const bf16x8 yf = slab_frag_tr(ytile, kChunk, t * 32, st, lane);
+    for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-      for (int i = 0; i < 3; ++i) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(yf, part[i], S[t], 0, 0, 0);
-    }
+      for (int t = 0; t < D / 32; ++t) S[t] = mfma(yf[t], part[i], S[t]);
   }
 }
 
@@ -201,47 +265,55 @@ __device__ __forceinline__ const T* rows_at(const void* base, long ld, int group
 }
 
 // ---------------------------------------------------------------------------
-// sums of the segments: parts[seg] = what the segment adds to the state that leaves it
+// sums of the segments: parts[seg] = what the segment adds to the state that leaves it.  Rows are weighted to the
+// segment's end, so the accumulators are only added to.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ __launch_bounds__(2 * D, 2) void linattn_sum_kernel(Params p) {
   using T = Tile<D>;
   constexpr int DT = D / 32;
-  __shared__ __align__(1024) uint8_t smem[2 * T::BYTES];
-  uint8_t* const ytile = smem;
-  uint8_t* const ztile = smem + T::BYTES;
+  extern __shared__ __align__(1024) uint8_t smem[];  // two stages of y and z, and the rows' weights of each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place w = place(p);
+  const Place w = place(p, p.n_sums);
   const Role& ro = p.role[w.role];
   // the last segment's sum enters the state that leaves the sequence and nothing else
   if (!ro.final_state && w.seg == (ro.reverse ? 0 : p.n_seg - 1)) return;
   const bf16_t* y = rows_at<bf16_t>(ro.y, ro.ldy, ro.gy, p, w, D);
   const bf16_t* z = rows_at<bf16_t>(ro.z, ro.ldz, ro.gz, p, w, D);
+  const uint32_t lds = lds_address(smem), unit = T::unit(), tr = tr_base(lane);
+  const uint32_t offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
   f32x16 S[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) S[t] = 0.f;
   const int n = (w.live + kChunk - 1) / kChunk;
-  uint4 ry[T::PER], rz[T::PER];
-  auto fetch = [&](int i) {
-    const int c = ro.reverse ? n - 1 - i : i;
-    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, w.live - c * kChunk);
-    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, w.live - c * kChunk);
+  typename T::Regs ry, rz;
+  auto fetch = [&](int c) {
+    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, offy, w.live - c * kChunk);
+    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, offz, w.live - c * kChunk);
   };
   if (n) fetch(0);
-  for (int i = 0; i < n; ++i) {
-    const int c = ro.reverse ? n - 1 - i : i;
-    T::put(ytile, ry);
-    T::put(ztile, rz);
-    __syncthreads();
-    if (i + 1 < n) fetch(i + 1);
+  for (int c = 0; c < n; ++c) {
+    const int rows = min(kChunk, w.live - c * kChunk);
+    const uint32_t ytile = lds + (c & 1) * (2 * T::BYTES + kChunk * 4), ztile = ytile + T::BYTES, up = ztile + T::BYTES;
+    // rows between this chunk and the end that the state leaves by
+    const int behind = ro.reverse ? c * kChunk : w.live - c * kChunk - rows;
+    if (threadIdx.x < kChunk) {
+      const int j = threadIdx.x;
+      lds_put(up + j * 4, ro.a_update * decay_pow(w.g2, behind + (ro.reverse ? j + 1 : max(rows - 1 - j, 0))));
+    }
+    T::put(ytile + unit, ry);
+    T::put(ztile + unit, rz);
+    __syncthreads();       // (and nobody is still reading the stage that the next trip fills)
+    if (c + 1 < n) fetch(c + 1);
     bf16x8 zf[4];
 #pragma unroll
-    for (int st = 0; st < 4; ++st) zf[st] = slab_frag_tr(ztile, kChunk, wave * 32, st, lane);
-    update_state<D>(S, ytile, zf, w.g2, ro.a_update, min(kChunk, w.live - c * kChunk), ro.reverse, lane);
-    __syncthreads();
+    for (int st = 0; st < 4; ++st) zf[st] = tr_frag(ztile + (wave >> 1) * 8192 + (tr ^ ((wave & 1) << 6)), 0, st);
+    update_state<D, 3>(S, ytile + tr, zf, up, lane);
   }
   store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
 }
+template <int D>
+constexpr int sum_lds() { return 2 * (2 * Tile<D>::BYTES + kChunk * 4); }
 
 // ---------------------------------------------------------------------------
 // carry: parts[seg] becomes the state that enters the segment; one thread per 4 elements of a state
@@ -252,8 +324,8 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
   unsigned i = blockIdx.x;
   const int e = ((i % BLOCKS) * 256 + threadIdx.x) * 4;
   i /= BLOCKS;
-  const Role& ro = p.role[i % p.n_roles];
-  const unsigned bh = i / p.n_roles;
+  const Role& ro = p.role[i % p.n_sums];
+  const unsigned bh = i / p.n_sums;
   const int h = bh % p.heads, b = bh / p.heads;
   const float g2 = log2_decay(p.decay, h);
   const int len = rows_of(p, b);
@@ -281,24 +353,29 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
 }
 
 // ---------------------------------------------------------------------------
-// the walk, bf16.  Per chunk: P^T = Y X^T in quadrants of 32 x 32 (weighted, rounded to bf16 in two parts,
-// shared through LDS); O^T = S^T X^T from the state's accumulators as they are, times the rows' decay,
-// plus Z^T P^T; then the state's update.
+// the walk, bf16.  Per chunk: P^T = Y X^T in quadrants of 32 x 32 (weighted, in two bf16 parts, shared through
+// LDS); O^T = S^T X^T from the state's accumulators as they are, times the rows' decay, plus Z^T P^T; then the
+// state's update.
 // The state and the pairs meet the matrix cores as two bf16 each (16 bits): one would add, to
 // the rounding of the result, as much again.
+// PARTS: of the state's terms, see update_state.
 // ---------------------------------------------------------------------------
 template <int D>
+constexpr int walk_lds() { return 3 * Tile<D>::BYTES + 2 * 8192 + (int)sizeof(Weights); }
+
+template <int D, int PARTS>
 __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
   using T = Tile<D>;
   constexpr int DT = D / 32, NW = D / 32;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* const xtile = smem;                       // later the chunk's result
-  uint8_t* const ytile = smem + T::BYTES;
-  uint8_t* const ztile = smem + 2 * T::BYTES;
-  uint8_t* const ptile = smem + 3 * T::BYTES;        // two parts of 8 KB, rows i, j in the accumulators' order
+  const uint32_t xtile = lds_address(smem);          // later the chunk's result
+  const uint32_t ytile = xtile + T::BYTES, ztile = ytile + T::BYTES;
+  const uint32_t ptile = ztile + T::BYTES;           // two parts of 8 KB, rows i, j in the accumulators' order
+  Weights* const weights = (Weights*)(smem + 3 * T::BYTES + 2 * 8192);
+  const uint32_t pair = lds_address(weights->pair), up = lds_address(weights->up), ofstate = lds_address(weights->state);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hh = lane >> 5, li = lane & 31;
-  const Place w = place(p);
+  const Place w = place(p, p.n_roles);
   const Role& ro = p.role[w.role];
   const bool rev = ro.reverse;
   const bf16_t* x = rows_at<bf16_t>(ro.x, ro.ldx, ro.gx, p, w, D);
@@ -309,99 +386,99 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
   f32x16 S[DT];
   const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
   if (from) {
-    load_state<D>(S, from, p.n_seg == 1 && ro.init_transposed, wave, lane);
+    load_state<D>(S, from, p.n_seg == 1 ? ro.init_transposed : ro.parts_transposed, wave, lane);
   } else {
 #pragma unroll
     for (int t = 0; t < DT; ++t) S[t] = 0.f;
   }
-  bool have_state = from != nullptr;
   const bool keep_last = p.n_seg == 1 && ro.final_state;
+  const uint32_t unit = T::unit(), tr = tr_base(lane);
+  const uint32_t row = slab_off(li, 0);              // unit c of row li (+ 32: 4096 further) is at row ^ c * 16
+  const uint32_t offx = T::offset(ro.ldx), offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
 
   const int n = (w.live + kChunk - 1) / kChunk;
-  uint4 rx[T::PER], ry[T::PER], rz[T::PER];
+  typename T::Regs rx, ry, rz;
   auto fetch = [&](int i) {
     const int c = rev ? n - 1 - i : i;
-    T::load(rx, x + (long)c * kChunk * ro.ldx, ro.ldx, w.live - c * kChunk);
-    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, w.live - c * kChunk);
-    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, w.live - c * kChunk);
+    T::load(rx, x + (long)c * kChunk * ro.ldx, ro.ldx, offx, w.live - c * kChunk);
+    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, offy, w.live - c * kChunk);
+    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, offz, w.live - c * kChunk);
   };
   if (n) fetch(0);
+  pair_weights(weights, w.g2, ro.a_pair, rev);
+  // the quadrant of pairs that never counts stays zero
+  for (int k = threadIdx.x; k < 256; k += T::THREADS) {
+    const int part = k >> 7, r = k & 31, c = (k >> 5) & 3;
+    lds_put(ptile + part * 8192 + (rev ? 4096 : 0) + slab_off(r, (rev ? 0 : 4) + c), u32x4{0, 0, 0, 0});
+  }
   for (int i = 0; i < n; ++i) {
     const int c = rev ? n - 1 - i : i;
     const int rows = min(kChunk, w.live - c * kChunk);
-    T::put(xtile, rx);
-    T::put(ytile, ry);
-    T::put(ztile, rz);
+    row_weights(weights, w.g2, ro.a_update, ro.a_state, rows, rev);
+    T::put(xtile + unit, rx);
+    T::put(ytile + unit, ry);
+    T::put(ztile + unit, rz);
     __syncthreads();
     if (i + 1 < n) fetch(i + 1);
 
 #pragma unroll
-    for (int q = wave; q < 4; q += NW) {
-      const int jt = q >> 1, it = q & 1;
+    for (int q = 0; q < 4 / NW; ++q) {
+      const int jt = q * (NW / 2) + (wave >> 1), it = wave & 1;
       if (rev ? jt < it : jt > it) continue;       // no pair of these rows counts
       f32x16 s;
       s = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(slabs_frag<D>(ytile, jt * 32, ks, lane),
-                                                    slabs_frag<D>(xtile, it * 32, ks, lane), s, 0, 0, 0);
-      const int row = it * 32 + li;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = jt * 32 + (r >> 2) * 8 + hh * 4 + (r & 3);
-        const int far = rev ? j - row : row - j;
-        s[r] = far >= 0 ? s[r] * (ro.a_pair * decay_pow(w.g2, max(far, 0))) : 0.f;
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint32_t at = (row ^ ((ks & 3) * 32 + hh * 16)) + (ks >> 2) * 8192;
+        s = mfma(lds_get<bf16x8>(ytile + jt * 4096 + at), lds_get<bf16x8>(xtile + it * 4096 + at), s);
       }
+      const uint32_t far = pair + (64 + (it - jt) * 32 + li - hh * 4 - 27) * 4;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= lds_get<float>(far + (27 - (r >> 2) * 8 - (r & 3)) * 4);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        f32x8 v = acc8(s, s2 * 8);
-#pragma unroll
-        for (int part = 0; part < 2; ++part)
-          *(bf16x8*)(ptile + part * 8192 + slab_off(row, (jt * 2 + s2) * 2 + hh)) = split(v);
+        float v[8];
+        acc8(v, s, s2 * 8);
+        const uint32_t at = ptile + it * 4096 + (row ^ ((jt * 2 + s2) * 32 + hh * 16));
+        lds_put(at, split(v));
+        lds_put(at + 8192, nearest(v));
       }
     }
 
     f32x16 o[2];
     o[0] = 0.f;
     o[1] = 0.f;
-    if (have_state) {
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-          f32x8 v = acc8(S[t], s2 * 8);
-          const bf16x8 hi = split(v), lo = split(v);
+      for (int s2 = 0; s2 < 2; ++s2) {
+        float v[8];
+        acc8(v, S[t], s2 * 8);
+        const bf16x8 hi = split(v), lo = nearest(v);
+        // elements 32 t + 16 s2 + 4 hh .. + 3 of the rows, and the same 8 further on
+        const uint32_t a = xtile + (row ^ ((t & 1) * 64 + s2 * 32)) + (t >> 1) * 8192 + hh * 8;
+        const uint32_t b = xtile + (row ^ ((t & 1) * 64 + s2 * 32 + 16)) + (t >> 1) * 8192 + hh * 8;
 #pragma unroll
-          for (int it = 0; it < 2; ++it) {
-            // row it * 32 + li, elements 32 t + 16 s2 + 4 hh .. + 3 and the same 8 further on
-            const int row = it * 32 + li, u = (t & 1) * 4 + s2 * 2;
-            const uint8_t* slab = xtile + (t >> 1) * 8192 + hh * 8;
-            const uint2 a = *(const uint2*)(slab + slab_off(row, u));
-            const uint2 b = *(const uint2*)(slab + slab_off(row, u + 1));
-            const bf16x8 xf = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y));
-            o[it] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, xf, o[it], 0, 0, 0);
-            o[it] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, xf, o[it], 0, 0, 0);
-          }
+        for (int it = 0; it < 2; ++it) {
+          const u32x2 first = lds_get<u32x2>(a + it * 4096), second = lds_get<u32x2>(b + it * 4096);
+          const bf16x8 xf = __builtin_bit_cast(bf16x8, u32x4{first.x, first.y, second.x, second.y});
+          o[it] = mfma(hi, xf, o[it]);
+          o[it] = mfma(lo, xf, o[it]);
         }
-#pragma unroll
-      for (int it = 0; it < 2; ++it) {
-        const int row = it * 32 + li;
-        o[it] *= ro.a_state * decay_pow(w.g2, rev ? max(rows - 1 - row, 0) : row + 1);
       }
-    }
+#pragma unroll
+    for (int it = 0; it < 2; ++it) o[it] *= lds_get<float>(ofstate + (it * 32 + li) * 4);
     bf16x8 zf[4];
 #pragma unroll
-    for (int st = 0; st < 4; ++st) zf[st] = slab_frag_tr(ztile, kChunk, wave * 32, st, lane);
+    for (int st = 0; st < 4; ++st) zf[st] = tr_frag(ztile + (wave >> 1) * 8192 + (tr ^ ((wave & 1) << 6)), 0, st);
     __syncthreads();
 #pragma unroll
-    for (int it = 0; it < 2; ++it)
+    for (int st = 0; st < 4; ++st)
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        if (rev ? (st >> 1) < it : (st >> 1) > it) continue;
+      for (int it = 0; it < 2; ++it) {
 #pragma unroll
         for (int part = 0; part < 2; ++part)
-          o[it] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(zf[st], slab_frag(ptile + part * 8192, it * 32, st, lane), o[it],
-                                                          0, 0, 0);
+          o[it] = mfma(zf[st], lds_get<bf16x8>(ptile + part * 8192 + it * 4096 + (row ^ (st * 32 + hh * 16))), o[it]);
       }
     if (ro.out_f32) {
       float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D + wave * 32;
@@ -417,30 +494,31 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
 #pragma unroll
       for (int it = 0; it < 2; ++it)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int u = wave * 4 + q;
-          *(uint2*)(xtile + (u >> 3) * 8192 + slab_off(it * 32 + li, u & 7) + hh * 8) =
-              make_uint2(pack2(o[it][4 * q], o[it][4 * q + 1]), pack2(o[it][4 * q + 2], o[it][4 * q + 3]));
-        }
+        for (int q = 0; q < 4; ++q)
+          lds_put(xtile + (wave >> 1) * 8192 + it * 4096 + (row ^ ((wave & 1) * 64 + q * 16)) + hh * 8,
+                  u32x2{pack2(o[it][4 * q], o[it][4 * q + 1]), pack2(o[it][4 * q + 2], o[it][4 * q + 3])});
     }
-    if (i + 1 < n || keep_last) update_state<D>(S, ytile, zf, w.g2, ro.a_update, rows, rev, lane);
-    have_state = true;
+    if (i + 1 < n || keep_last) {
+      const float keep = decay_pow(w.g2, rows);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) S[t] *= keep;
+      update_state<D, PARTS>(S, ytile + tr, zf, up, lane);
+    }
     __syncthreads();
     if (!ro.out_f32) {
-      bf16_t* out = (bf16_t*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D;
+      uint8_t* out = (uint8_t*)((bf16_t*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D);
+      const uint32_t off = T::offset(ro.ldo);
 #pragma unroll
-      for (int k = 0; k < T::PER; ++k) {
-        const int u = k * T::THREADS + threadIdx.x, row = u / T::UNITS, col = u % T::UNITS;
+      for (int k = 0; k < T::PER; ++k)
         // (the unit this thread overwrites with the next chunk's x)
-        if (row < rows) *(uint4*)(out + row * ro.ldo + col * 8) = *(const uint4*)T::unit(xtile, k);
-      }
+        if ((int)(threadIdx.x / T::UNITS) + 16 * k < rows) *(u32x4*)(out + 32 * k * ro.ldo + off) = lds_get<u32x4>(xtile + unit + k * 2048);
     }
   }
   if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
   // rows behind the sequence's end
-  const int unit = ro.out_f32 ? 4 : 8, units = D / unit;
+  const int per = ro.out_f32 ? 4 : 8, units = D / per;
   for (int k = threadIdx.x; k < (w.s1 - w.s0 - w.live) * units; k += T::THREADS) {
-    const long at = ((long)w.b * p.seq + w.s0 + w.live + k / units) * ro.ldo + (long)(w.h / ro.go) * D + (k % units) * unit;
+    const long at = ((long)w.b * p.seq + w.s0 + w.live + k / units) * ro.ldo + (long)(w.h / ro.go) * D + (k % units) * per;
     *(uint4*)((uint8_t*)ro.out + at * (ro.out_f32 ? 4 : 2)) = make_uint4(0, 0, 0, 0);
   }
 }
@@ -498,7 +576,7 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_sum_f32_kernel(Params p) {
   float* const ytile = smem;
   float* const ztile = smem + kChunkF32 * T::LD;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place w = place(p);
+  const Place w = place(p, p.n_sums);
   const Role& ro = p.role[w.role];
   if (!ro.final_state && w.seg == (ro.reverse ? 0 : p.n_seg - 1)) return;
   const float* y = rows_at<float>(ro.y, ro.ldy, ro.gy, p, w, D);
@@ -540,7 +618,7 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_f32_kernel(Params p) {
   float* const ztile = smem + 2 * kChunkF32 * T::LD;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hh = lane >> 5, li = lane & 31;
-  const Place w = place(p);
+  const Place w = place(p, p.n_roles);
   const Role& ro = p.role[w.role];
   const bool rev = ro.reverse;
   const float* x = rows_at<float>(ro.x, ro.ldx, ro.gx, p, w, D);
@@ -551,7 +629,7 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_f32_kernel(Params p) {
   f32x16 S[DT];
   const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
   if (from) {
-    load_state<D>(S, from, p.n_seg == 1 && ro.init_transposed, wave, lane);
+    load_state<D>(S, from, p.n_seg == 1 ? ro.init_transposed : ro.parts_transposed, wave, lane);
   } else {
 #pragma unroll
     for (int t = 0; t < DT; ++t) S[t] = 0.f;
@@ -711,16 +789,29 @@ __global__ __launch_bounds__(256) void linattn_step_kernel(const E* q, const E* 
 // host
 // ---------------------------------------------------------------------------
 constexpr int kSegUnit = 128;      // rows a segment is a multiple of
-constexpr int kWantWorkgroups = 512;
+constexpr int kMaxSegments = 64;
 
-// Rows of a segment for `walks` sequences x heads x roles: one segment if they fill the device, else as
-// many as bring two workgroups to a CU.
-int segment_rows(int64_t walks, int64_t seq) {
-  if (walks >= kWantWorkgroups || seq <= 2 * kSegUnit) return (int)std::max<int64_t>(seq, 1);
-  const int64_t segs = (kWantWorkgroups + walks - 1) / walks;
-  const int64_t rows = (seq + segs - 1) / segs;
-  const int64_t unit = (rows + kSegUnit - 1) / kSegUnit * kSegUnit;
-  return (int)std::min<int64_t>(unit, seq);
+// Workgroups that run at a time: by their LDS and registers two to a CU with heads of 128; with heads of 64, whose
+// workgroups have half the waves, three (bf16) or four (f32).
+int slots_of(int head_dim, bool f32) { return 256 * (head_dim == 128 ? 2 : f32 ? 4 : 3); }
+
+// Rows of a segment for `walks` sequences x heads x roles.  A cut costs every segment the state's way in and out and a
+// pass over two of its three operands; it pays where whole rounds of workgroups get shorter by it.
+int segment_rows(int64_t walks, int64_t seq, int slots) {
+  int64_t best = std::max<int64_t>(seq, 1);
+  double least = 0;
+  for (int n = 1; n <= kMaxSegments; ++n) {
+    const int64_t rows = n == 1 ? std::max<int64_t>(seq, 1) : (seq + n * kSegUnit - 1) / (n * kSegUnit) * kSegUnit;
+    const int64_t segs = (seq + rows - 1) / rows;
+    const double rounds = (double)((walks * segs + slots - 1) / slots);
+    const double time = rounds * (n == 1 ? rows + 64. : 1.6 * rows + 256.) + (n == 1 ? 0. : 256.);
+    if (n == 1 || time < least) {
+      least = time;
+      best = rows;
+    }
+    if (rows <= kSegUnit) break;
+  }
+  return (int)best;
 }
 
 struct Split {
@@ -730,7 +821,7 @@ struct Split {
 };
 Split split_of(const jpp_linattn_args* a, int roles) {
   Split s;
-  s.rows = segment_rows((int64_t)a->batch * a->n_heads * roles, a->seq);
+  s.rows = segment_rows((int64_t)a->batch * a->n_heads * roles, a->seq, slots_of(a->head_dim, a->dtype == JPP_DTYPE_F32));
   s.n = std::max(1, (a->seq + s.rows - 1) / s.rows);     // (no rows: a walk that hands the state on)
   const size_t states = (size_t)a->batch * a->n_heads * a->head_dim * a->head_dim * 4;
   s.parts = s.n > 1 ? states * s.n : 0;
@@ -757,6 +848,7 @@ int check_tensor(const void* p, int64_t ld, int heads, int rows, const jpp_linat
   if (rows == 0) return JPP_OK;      // nothing of it is touched
   JPP_REQUIRE(p, "%s: null operand %s", who, name);
   JPP_REQUIRE(ld >= (int64_t)heads * a->head_dim, "%s: leading dimension of %s too small", who, name);
+  JPP_REQUIRE(ld < (1 << 26), "%s: leading dimension of %s too large", who, name);   // 16 rows in 32 bits of bytes
   JPP_REQUIRE(ld % unit == 0 && (uintptr_t)p % 16 == 0, "%s: %s must keep 16-byte alignment", who, name);
   return JPP_OK;
 }
@@ -772,11 +864,16 @@ int check_state(const void* p, const char* who, const char* name) {
 
 template <int D, bool F32>
 int launch(hipStream_t st, const Params& p) {
-  const int64_t walks = (int64_t)p.batch * p.heads * p.n_roles;
+  const int64_t walks = (int64_t)p.batch * p.heads * p.n_roles, sums = (int64_t)p.batch * p.heads * p.n_sums;
   if (p.n_seg > 1) {
-    const unsigned carry = (unsigned)(walks * (D * D / 1024));
-    if constexpr (F32) hipLaunchKernelGGL((linattn_sum_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), 0, st, p);
-    else hipLaunchKernelGGL((linattn_sum_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), 0, st, p);
+    const unsigned carry = (unsigned)(sums * (D * D / 1024));
+    const dim3 grid((unsigned)(sums * p.n_seg));
+    if constexpr (F32) {
+      hipLaunchKernelGGL((linattn_sum_f32_kernel<D>), grid, dim3(2 * D), 0, st, p);
+    } else {
+      JPP_TRY(jpp_attn::set_smem(linattn_sum_kernel<D>, sum_lds<D>()));
+      hipLaunchKernelGGL((linattn_sum_kernel<D>), grid, dim3(2 * D), sum_lds<D>(), st, p);
+    }
     JPP_LAUNCH_CHECK();
     hipLaunchKernelGGL((linattn_carry_kernel<D>), dim3(carry), dim3(256), 0, st, p);
     JPP_LAUNCH_CHECK();
@@ -784,9 +881,16 @@ int launch(hipStream_t st, const Params& p) {
   if constexpr (F32) {
     hipLaunchKernelGGL((linattn_walk_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), 0, st, p);
   } else {
-    constexpr int kLds = 3 * Tile<D>::BYTES + 2 * 8192;
-    if (kLds > 64 * 1024) JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D>, kLds));
-    hipLaunchKernelGGL((linattn_walk_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), kLds, st, p);
+    bool last = false;           // a state that is a result comes out of the walk
+    for (int i = 0; i < p.n_roles; ++i) last = last || (p.n_seg == 1 && p.role[i].final_state);
+    const dim3 grid((unsigned)(walks * p.n_seg));
+    if (last) {
+      JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 3>, walk_lds<D>()));
+      hipLaunchKernelGGL((linattn_walk_kernel<D, 3>), grid, dim3(2 * D), walk_lds<D>(), st, p);
+    } else {
+      JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 2>, walk_lds<D>()));
+      hipLaunchKernelGGL((linattn_walk_kernel<D, 2>), grid, dim3(2 * D), walk_lds<D>(), st, p);
+    }
   }
   JPP_LAUNCH_CHECK();
   return JPP_OK;
@@ -818,7 +922,7 @@ double flops_of(const jpp_linattn_args* a) {
 extern "C" size_t jpp_linattn_workspace_bytes(const jpp_linattn_args* a, int backward) {
   if (check_sizes(a, "linattn_workspace_bytes") || a->batch == 0 || a->seq == 0) return 0;
   const Split s = split_of(a, backward ? 3 : 1);
-  return backward ? 3 * s.parts + 2 * s.groups : s.parts;
+  return backward ? 2 * s.parts + 2 * s.groups : s.parts;
 }
 
 extern "C" int jpp_linattn_fwd(void* stream, const jpp_linattn_args* a) {
@@ -838,8 +942,8 @@ extern "C" int jpp_linattn_fwd(void* stream, const jpp_linattn_args* a) {
   JPP_TRY(check_state(a->workspace, who, "workspace"));
   const int group = a->n_heads / a->n_kv_heads;
   Params p = params_of(a, s);
-  p.n_roles = 1;
-  p.role[0] = {a->q, a->k, a->v, a->o, a->ldq, a->ldk, a->ldv, a->ldo, 1, group, group, 1, 0, 0, 0,
+  p.n_roles = p.n_sums = 1;
+  p.role[0] = {a->q, a->k, a->v, a->o, a->ldq, a->ldk, a->ldv, a->ldo, 1, group, group, 1, 0, 0, 0, 0,
                a->scale, a->scale, 1.f, a->state_in, a->state_out, (float*)a->workspace};
   const double es = a->dtype == JPP_DTYPE_F32 ? 4 : 2;
   ProbeScope probe((hipStream_t)stream, "linattn_fwd", 2 * flops_of(a),
@@ -869,24 +973,25 @@ extern "C" int jpp_linattn_bwd(void* stream, const jpp_linattn_args* a) {
   JPP_REQUIRE(!a->d_state_in || (a->d_state_in != a->state_in && a->d_state_in != a->d_state_out),
               "%s: d_state_in overlaps an input", who);
   const Split s = split_of(a, 3);
-  JPP_REQUIRE(s.parts + s.groups == 0 || a->workspace, "%s: workspace of %zu bytes wanted", who, 3 * s.parts + 2 * s.groups);
+  JPP_REQUIRE(s.parts + s.groups == 0 || a->workspace, "%s: workspace of %zu bytes wanted", who, 2 * s.parts + 2 * s.groups);
   JPP_TRY(check_state(a->workspace, who, "workspace"));
   const int group = a->n_heads / a->n_kv_heads, f32 = a->dtype == JPP_DTYPE_F32;
   const long wide = (long)a->n_heads * a->head_dim;
   uint8_t* ws = (uint8_t*)a->workspace;
-  float* parts[3];
-  for (int i = 0; i < 3; ++i) parts[i] = (float*)(ws + i * s.parts);
-  float* dk_parts = (float*)(ws + 3 * s.parts);
-  float* dv_parts = (float*)(ws + 3 * s.parts + s.groups);
+  float* const s_parts = (float*)ws;
+  float* const u_parts = (float*)(ws + s.parts);
+  float* const dk_parts = (float*)(ws + 2 * s.parts);
+  float* const dv_parts = (float*)(ws + 2 * s.parts + s.groups);
   const bool shared = s.groups != 0;
   Params p = params_of(a, s);
   p.n_roles = 3;
-  p.role[0] = {a->d_o, a->v, a->k, a->dq, a->lddo, a->ldv, a->ldk, a->lddq, 1, group, group, 1, 0, 1, 0,
-               a->scale, a->scale, 1.f, a->state_in, nullptr, parts[0]};
-  p.role[1] = {a->v, a->d_o, a->q, shared ? (void*)dk_parts : a->dk, a->ldv, a->lddo, a->ldq, shared ? wide : (long)a->lddk,
-               group, 1, 1, 1, 1, 1, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, nullptr, parts[1]};
-  p.role[2] = {a->k, a->q, a->d_o, shared ? (void*)dv_parts : a->dv, a->ldk, a->ldq, a->lddo, shared ? wide : (long)a->lddv,
-               group, 1, 1, 1, 1, 0, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, a->d_state_in, parts[2]};
+  p.n_sums = 2;
+  p.role[0] = {a->d_o, a->v, a->k, a->dq, a->lddo, a->ldv, a->ldk, a->lddq, 1, group, group, 1, 0, 1, 0, 0,
+               a->scale, a->scale, 1.f, a->state_in, nullptr, s_parts};
+  p.role[1] = {a->k, a->q, a->d_o, shared ? (void*)dv_parts : a->dv, a->ldk, a->ldq, a->lddo, shared ? wide : (long)a->lddv,
+               group, 1, 1, 1, 1, 0, 0, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, a->d_state_in, u_parts};
+  p.role[2] = {a->v, a->d_o, a->q, shared ? (void*)dk_parts : a->dk, a->ldv, a->lddo, a->ldq, shared ? wide : (long)a->lddk,
+               group, 1, 1, 1, 1, 1, 1, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, nullptr, u_parts};
   hipStream_t st = (hipStream_t)stream;
   const double es = f32 ? 4 : 2;
   ProbeScope probe(st, "linattn_bwd", 5 * flops_of(a),

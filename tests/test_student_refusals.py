@@ -41,7 +41,7 @@ def test_linear_attention(change, match):
 def test_linear_attention_operands_of_each_direction():
     _refused("jpp_linattn_fwd", _lin(o=None), "o", None)
     _refused("jpp_linattn_fwd", _lin(o=3 * AT), "overlaps", None)
-    _refused("jpp_linattn_fwd", _lin(workspace=None), "workspace", None)
+    _refused("jpp_linattn_fwd", _lin(workspace=None, seq=4096), "workspace", None)
     _refused("jpp_linattn_fwd", _lin(state_in=AT + 4), "state_in", None)
     _refused("jpp_linattn_fwd", _lin(dtype=1, ldo=258), "alignment", None)
     _refused("jpp_linattn_bwd", _lin(d_o=None), "d_o", None)
