@@ -44,10 +44,12 @@ template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  if constexpr (TPR == 256) {
+  if constexpr (TPR > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = red[0] + red[1] + red[2] + red[3];
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 64; ++i) v += red[i];
   }
   return v;
 }
@@ -135,111 +137,140 @@ __global__ __launch_bounds__(256) void block_join_fwd_kernel(JoinParams p) {
 }
 
 // Workgroup `part` of a gate row's `splits`: its share of that row's rows, and one line of the sums E and F over them.
-template <class E, int TPR, int NCH>
-__global__ __launch_bounds__(256) void block_join_bwd_kernel(JoinParams p) {
-  constexpr int N = Unit<E>::N, LANES = 256 / TPR;
-  extern __shared__ float lds[];      // 16 floats of reductions (TPR = 256), or 2 x LANES x cols sums (TPR = 64)
+// The next row's operands are on their way while a row is worked on.
+constexpr int bwd_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+
+template <class E, int TPR, int NCH, bool PRE, bool POST>
+__global__ __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 4 : 2) void block_join_bwd_kernel(JoinParams p) {
+  constexpr int N = Unit<E>::N, LANES = bwd_threads(TPR) / TPR;
+  extern __shared__ float lds[];      // 64 floats of reductions (TPR > 64), or 2 x LANES x cols sums (TPR = 64)
   const int t = threadIdx.x % TPR, lane = threadIdx.x / TPR;
   const int units = p.cols / N;
-  const long group = blockIdx.x / p.splits, part = blockIdx.x % p.splits;
+  const long group = blockIdx.x / (unsigned)p.splits, part = blockIdx.x % (unsigned)p.splits;
   const long per = (p.gate_rows + p.splits - 1) / p.splits;
   const long first = group * p.gate_rows + part * per;
   const long last = min(min(first + per, (group + 1) * p.gate_rows), p.rows);
   const uint4* gr = p.gate ? (const uint4*)((const E*)p.gate + group * p.cols) : nullptr;
+  const bool with_dh = p.dh != nullptr;
   float se[NCH][N], sf[NCH][N];
 #pragma unroll
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
     for (int e = 0; e < N; ++e) se[i][e] = sf[i][e] = 0.f;
-  int turn = 0;
-  for (long row = first + lane; row < last; row += LANES, turn ^= 8) {
+  uint4 nb[NCH], nh[NCH], ny[NCH], nd[NCH];
+  float nrh = 0.f, nrb = 1.f;
+  auto fetch = [&](long row) {
     const long at = row * p.cols;
-    float total[NCH][N];
-    const float rh = p.gamma_pre ? p.rstd_pre[row] : 0.f;
-    const float rb = p.gamma_post ? p.rstd_post[row] : 1.f;
-    uint4 vb[NCH], vh[NCH], vy[NCH];
+    if (PRE) nrh = p.rstd_pre[row];
+    if (POST) nrb = p.rstd_post[row];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int c = t + TPR * i;
-      const bool in = c < units;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      vb[i] = in ? ((const uint4*)((const E*)p.b + at))[c] : zero;
-      vh[i] = in && p.gamma_pre ? ((const uint4*)((const E*)p.h + at))[c] : zero;
-      vy[i] = in && p.gamma_pre ? ((const uint4*)((const E*)p.dy + at))[c] : zero;
-      Unit<E>::get(in && p.dh ? ((const uint4*)((const E*)p.dh + at))[c] : zero, total[i]);
+      if (c < units) {
+        nb[i] = ((const uint4*)((const E*)p.b + at))[c];
+        if (PRE) nh[i] = ((const uint4*)((const E*)p.h + at))[c];
+        if (PRE) ny[i] = ((const uint4*)((const E*)p.dy + at))[c];
+        if (with_dh) nd[i] = ((const uint4*)((const E*)p.dh + at))[c];
+      }
     }
-    if (p.gamma_pre) {
-      float s = 0.f;
+  };
+  // (units beyond the row stay zero and add nothing)
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) nb[i] = nh[i] = ny[i] = nd[i] = make_uint4(0, 0, 0, 0);
+  if (first + lane < last) fetch(first + lane);
+  int turn = 0;
+  for (long row = first + lane; row < last; row += LANES, turn ^= 32) {
+    const long at = row * p.cols;
+    const float rh = nrh, rb = nrb;
+    uint4 vb[NCH];
+    float total[NCH][N];
+    float s = 0.f;
+    if (PRE) {
+      uint4 vh[NCH], vy[NCH];
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        vb[i] = nb[i];
+        vh[i] = nh[i];
+        vy[i] = ny[i];
+        Unit<E>::get(nd[i], total[i]);
+      }
+      if (row + LANES < last) fetch(row + LANES);
+      uint4 vw[NCH];
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         const int c = t + TPR * i;
-        if (c < units) {
-          float w[N], h[N], y[N];
-          Unit<E>::get(((const uint4*)p.gamma_pre)[c], w);
-          Unit<E>::get(vh[i], h);
-          Unit<E>::get(vy[i], y);
+        vw[i] = make_uint4(0, 0, 0, 0);
+        if (c < units) vw[i] = ((const uint4*)p.gamma_pre)[c];
+        float w[N], h[N], y[N];
+        Unit<E>::get(vw[i], w);
+        Unit<E>::get(vh[i], h);
+        Unit<E>::get(vy[i], y);
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            s += y[e] * w[e] * (h[e] * rh);
-            sf[i][e] += y[e] * (h[e] * rh);
-          }
+        for (int e = 0; e < N; ++e) {
+          const float yh = y[e] * (h[e] * rh);
+          s += yh * w[e];
+          sf[i][e] += yh;
         }
       }
       s = row_sum<TPR>(s, lds + turn) / p.cols;
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const int c = t + TPR * i;
-        if (c < units) {
-          float w[N], h[N], y[N];
-          Unit<E>::get(((const uint4*)p.gamma_pre)[c], w);
-          Unit<E>::get(vh[i], h);
-          Unit<E>::get(vy[i], y);
+        float w[N], h[N], y[N];
+        Unit<E>::get(vw[i], w);
+        Unit<E>::get(vh[i], h);
+        Unit<E>::get(vy[i], y);
 #pragma unroll
-          for (int e = 0; e < N; ++e) total[i][e] += rh * (y[e] * w[e] - h[e] * rh * s);
-        }
+        for (int e = 0; e < N; ++e) total[i][e] += rh * (y[e] * w[e] - h[e] * rh * s);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        vb[i] = nb[i];
+        Unit<E>::get(nd[i], total[i]);
+      }
+      if (row + LANES < last) fetch(row + LANES);
     }
-    float u[NCH][N], s = 0.f;
+    s = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int c = t + TPR * i;
-      float b[N], w[N];
+      float b[N], dx[N], w[N];
       Unit<E>::get(vb[i], b);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        se[i][e] += total[i][e] * (b[e] * rb);
-        u[i][e] = total[i][e];
+        dx[e] = p.alpha * total[i][e];
+        if (POST) b[e] *= rb;
+        se[i][e] += total[i][e] * b[e];
       }
       if (c < units) {
+        ((uint4*)((E*)p.dx + at))[c] = Unit<E>::put(dx);
         if (gr) {
           Unit<E>::get(gr[c], w);
 #pragma unroll
-          for (int e = 0; e < N; ++e) u[i][e] *= w[e];
+          for (int e = 0; e < N; ++e) total[i][e] *= w[e];
         }
-        if (p.gamma_post) {
+        if (POST) {
           Unit<E>::get(((const uint4*)p.gamma_post)[c], w);
 #pragma unroll
           for (int e = 0; e < N; ++e) {
-            u[i][e] *= w[e];
-            s += u[i][e] * (b[e] * rb);
+            total[i][e] *= w[e];
+            s += total[i][e] * b[e];
           }
         }
-#pragma unroll
-        for (int e = 0; e < N; ++e) total[i][e] *= p.alpha;
       }
     }
-    if (p.gamma_post) s = row_sum<TPR>(s, lds + turn + 4) / p.cols;
+    if (POST) s = row_sum<TPR>(s, lds + turn + 16) / p.cols;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int c = t + TPR * i;
       if (c < units) {
-        float b[N];
-        Unit<E>::get(vb[i], b);
-        if (p.gamma_post)
+        if (POST) {
+          float b[N];
+          Unit<E>::get(vb[i], b);
 #pragma unroll
-          for (int e = 0; e < N; ++e) u[i][e] = rb * (u[i][e] - b[e] * rb * s);
-        ((uint4*)((E*)p.dx + at))[c] = Unit<E>::put(total[i]);
-        ((uint4*)((E*)p.db + at))[c] = Unit<E>::put(u[i]);
+          for (int e = 0; e < N; ++e) total[i][e] = rb * (total[i][e] - b[e] * rb * s);
+        }
+        ((uint4*)((E*)p.db + at))[c] = Unit<E>::put(total[i]);
       }
     }
   }
@@ -251,9 +282,9 @@ __global__ __launch_bounds__(256) void block_join_bwd_kernel(JoinParams p) {
       const int c = t + TPR * i;
       if (c < units)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          p.sum_e[line + c * N + e] = se[i][e];
-          p.sum_f[line + c * N + e] = sf[i][e];
+        for (int e = 0; e < N; e += 4) {
+          *(float4*)(p.sum_e + line + c * N + e) = make_float4(se[i][e], se[i][e + 1], se[i][e + 2], se[i][e + 3]);
+          *(float4*)(p.sum_f + line + c * N + e) = make_float4(sf[i][e], sf[i][e + 1], sf[i][e + 2], sf[i][e + 3]);
         }
     }
   } else {
@@ -281,49 +312,59 @@ __global__ __launch_bounds__(256) void block_join_bwd_kernel(JoinParams p) {
   }
 }
 
-// The lines' sums, in their order: 32 columns by 32 shares of the lines.  blockIdx.y = 0: dgamma_pre and
-// dgamma_post; beyond: dgate.
+// The lines' sums, in a fixed order: 32 columns by 32 shares of the lines.  blockIdx.y = 0: dgamma_pre; 1: dgamma_post;
+// beyond: dgate.
 template <class E>
 __global__ __launch_bounds__(1024) void block_join_sums_kernel(const float* sum_e, const float* sum_f, const E* gamma_post,
                                                                const E* gate, float* dgamma_pre, float* dgamma_post,
-                                                               float* dgate, int cols, long groups, int splits,
+                                                               float* dgate, int cols, int groups, int splits,
                                                                int accumulate) {
-  __shared__ float red[2][32][33];
+  __shared__ float red[32][33];
   const int c = threadIdx.x & 31, l = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
   const bool in = col < cols;
   auto value = [](const E* p) {
     if constexpr (sizeof(E) == 2) return bf16_to_f32(*p);
     else return *p;
   };
-  auto leave = [&](float* to, float v) { *to = accumulate ? *to + v : v; };
-  auto fold = [&](int k) {          // sum over the shares, in order
-    float v = 0.f;
-    for (int i = 0; i < 32; ++i) v += red[k][i][c];
-    return v;
-  };
-  if (blockIdx.y == 0) {
-    float a = 0.f, f = 0.f;
-    if (in)
-      for (long line = l; line < groups * splits; line += 32) {
-        const float e = sum_e[line * cols + col];
-        a += gate ? e * value(gate + line / splits * cols + col) : e;
-        f += sum_f[line * cols + col];
-      }
-    red[0][l][c] = a;
-    red[1][l][c] = f;
+  auto finish = [&](float v, float* to, float factor) {     // over the shares: a wave folds 2 columns' 32
     __syncthreads();
-    if (in && l == 0 && dgamma_post) leave(dgamma_post + col, fold(0));
-    if (in && l == 1 && dgamma_pre) leave(dgamma_pre + col, fold(1));
+    red[c][l] = v;
+    __syncthreads();
+    float sum = red[threadIdx.x >> 5][threadIdx.x & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    const int mine = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + mine < cols) {
+      float* at = to + blockIdx.x * 32 + mine;
+      if (gamma_post && factor == 0.f) sum *= value(gamma_post + blockIdx.x * 32 + mine);
+      *at = accumulate ? *at + sum : sum;
+    }
+  };
+  if (blockIdx.y < 2) {
+    float* to = blockIdx.y ? dgamma_post : dgamma_pre;
+    if (!to) return;
+    const float* from = blockIdx.y ? sum_e : sum_f;
+    const int lines = groups * splits;
+    float a = 0.f;
+    if (in) {
+      if (blockIdx.y && gate) {
+#pragma unroll 4
+        for (int line = l; line < lines; line += 32)
+          a += from[(long)line * cols + col] * value(gate + (long)(line / splits) * cols + col);
+      } else {
+#pragma unroll 8
+        for (int line = l; line < lines; line += 32) a += from[(long)line * cols + col];
+      }
+    }
+    finish(a, to, 1.f);
     return;
   }
-  for (long g = blockIdx.y - 1; g < groups; g += gridDim.y - 1) {
+  for (int g = blockIdx.y - 2; g < groups; g += gridDim.y - 2) {
     float a = 0.f;
     if (in)
-      for (int s = l; s < splits; s += 32) a += sum_e[(g * splits + s) * cols + col];
-    __syncthreads();
-    red[0][l][c] = a;
-    __syncthreads();
-    if (in && l == 0) leave(dgate + g * cols + col, fold(0) * (gamma_post ? value(gamma_post + col) : 1.f));
+#pragma unroll 4
+      for (int s = l; s < splits; s += 32) a += sum_e[((long)g * splits + s) * cols + col];
+    finish(a, dgate + (long)g * cols, 0.f);
   }
 }
 
@@ -367,25 +408,40 @@ JoinParams params_of(const jpp_join_args* a) {
   return p;
 }
 
-// Threads of a row and units of each: a wave up to two units a lane, a workgroup beyond.
-#define JPP_JOIN_BY_COLS(LAUNCH, E_)                                         \
-  do {                                                                       \
-    const int units_ = p.cols / Unit<E_>::N;                                 \
-    if (units_ <= 64) LAUNCH(E_, 64, 1);                                     \
-    else if (units_ <= 128) LAUNCH(E_, 64, 2);                               \
-    else if (units_ <= 256) LAUNCH(E_, 256, 1);                              \
-    else if (units_ <= 512) LAUNCH(E_, 256, 2);                              \
-    else if (units_ <= 1024) LAUNCH(E_, 256, 4);                             \
-    else if constexpr (Unit<E_>::N == 4) LAUNCH(E_, 256, 8);                 \
-  } while (0)
-
+// Threads of a row and units of each.  Forward: a wave up to two units a lane, 256 threads beyond.
 template <class E>
 int forward(hipStream_t st, const JoinParams& p) {
-#define JPP_JF(E_, T_, C_)                                                                                              \
-  hipLaunchKernelGGL((block_join_fwd_kernel<E_, T_, C_>), dim3((unsigned)((p.rows + 256 / T_ - 1) / (256 / T_))),       \
+  const int units = p.cols / Unit<E>::N;
+#define JPP_JF(T_, C_)                                                                                                  \
+  hipLaunchKernelGGL((block_join_fwd_kernel<E, T_, C_>), dim3((unsigned)((p.rows + 256 / T_ - 1) / (256 / T_))),        \
                      dim3(256), 0, st, p)
-  JPP_JOIN_BY_COLS(JPP_JF, E);
+  if (units <= 64) JPP_JF(64, 1);
+  else if (units <= 128) JPP_JF(64, 2);
+  else if (units <= 256) JPP_JF(256, 1);
+  else if (units <= 512) JPP_JF(256, 2);
+  else if (units <= 1024) JPP_JF(256, 4);
+  else if constexpr (Unit<E>::N == 4) JPP_JF(256, 8);
 #undef JPP_JF
+  JPP_LAUNCH_CHECK();
+  return JPP_OK;
+}
+
+// Backward: one unit a thread, so that a row, the next row and the sums fit the registers of twice the waves (8192 rows of
+// 8192 bf16: 187 us with 1024 threads of one unit, 204 with 512 of two and half the waves on a CU, 540 and more with
+// 256 of four, which spill).
+template <class E, bool PRE, bool POST>
+int backward_rows(hipStream_t st, const JoinParams& p, long lines) {
+  const int units = p.cols / Unit<E>::N;
+#define JPP_JB(T_, C_)                                                                                                 \
+  hipLaunchKernelGGL((block_join_bwd_kernel<E, T_, C_, PRE, POST>), dim3((unsigned)lines), dim3(bwd_threads(T_)),      \
+                     T_ > 64 ? 256 : 2 * (256 / T_) * p.cols * 4, st, p)
+  if (units <= 64) JPP_JB(64, 1);
+  else if (units <= 128) JPP_JB(64, 2);
+  else if (units <= 256) JPP_JB(256, 1);
+  else if (units <= 512) JPP_JB(512, 1);
+  else if (units <= 1024) JPP_JB(1024, 1);
+  else if constexpr (Unit<E>::N == 4) JPP_JB(1024, 2);
+#undef JPP_JB
   JPP_LAUNCH_CHECK();
   return JPP_OK;
 }
@@ -397,16 +453,14 @@ int backward(hipStream_t st, JoinParams p, const jpp_join_args* a) {
   p.splits = (int)std::min<long>(groups >= kJoinParts ? 1 : (kJoinParts + groups - 1) / groups, p.gate_rows);
   p.sum_e = sums ? (float*)a->workspace : nullptr;
   p.sum_f = sums ? p.sum_e + groups * p.splits * p.cols : nullptr;
-#define JPP_JB(E_, T_, C_)                                                                                          \
-  hipLaunchKernelGGL((block_join_bwd_kernel<E_, T_, C_>), dim3((unsigned)(groups * p.splits)), dim3(256),           \
-                     T_ == 256 ? 64 : 2 * (256 / T_) * p.cols * 4, st, p)
-  JPP_JOIN_BY_COLS(JPP_JB, E);
-#undef JPP_JB
-  JPP_LAUNCH_CHECK();
+  const long lines = groups * p.splits;
+  if (int rc = p.gamma_pre ? (p.gamma_post ? backward_rows<E, true, true>(st, p, lines) : backward_rows<E, true, false>(st, p, lines))
+                           : (p.gamma_post ? backward_rows<E, false, true>(st, p, lines) : backward_rows<E, false, false>(st, p, lines)))
+    return rc;
   if (!sums) return JPP_OK;
-  const dim3 grid((p.cols + 31) / 32, 1 + (unsigned)(a->dgate ? std::min<long>(groups, 4096) : 0));
+  const dim3 grid((p.cols + 31) / 32, 2 + (unsigned)(a->dgate ? std::min<long>(groups, 4096) : 0));
   hipLaunchKernelGGL((block_join_sums_kernel<E>), grid, dim3(1024), 0, st, p.sum_e, p.sum_f, (const E*)p.gamma_post,
-                     (const E*)p.gate, a->dgamma_pre, a->dgamma_post, a->dgate, p.cols, groups, p.splits, a->accumulate);
+                     (const E*)p.gate, a->dgamma_pre, a->dgamma_post, a->dgate, p.cols, (int)groups, p.splits, a->accumulate);
   JPP_LAUNCH_CHECK();
   return JPP_OK;
 }
