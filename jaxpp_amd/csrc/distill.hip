@@ -3,9 +3,10 @@
 //   p = softmax(teacher / T) over the listed ids,  q = softmax(z / T) over the vocabulary
 //   row_loss = w T^2 sum_k p_k (log p_k - log q_k),   dz = scale w T (q - p)
 //
-// HBM-bound: the logits are read, their gradient is written.  One workgroup per row: the running maximum and
-// sum of the softmax in one pass over the row, q in a second (which finds the row in the caches); the few listed
-// places are written last, each by one thread, so the sums do not depend on timing.
+// HBM-bound: the logits are read, their gradient is written.  One workgroup per row: the running maximum and sum of the
+// softmax in one pass over the row, q in a second, which finds the first units in registers and the others in the
+// caches.  Where rows are fewer than CUs they are cut into pieces: a launch that takes each piece's maximum and sum, and one
+// that joins them and writes.  The few listed places are written last, each by one thread, so no result depends on timing.
 #include <math.h>
 
 #include <algorithm>
@@ -56,148 +57,435 @@ __device__ __forceinline__ uint4 pack(const float (&f)[16 / sizeof(E)]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 }
 
-// over a workgroup of T threads; every thread gets the result.  `red`: T / 64 floats of LDS.
-template <int T, class F>
-__device__ __forceinline__ float reduce(float v, float* red, F&& f) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// over a workgroup of T threads; every thread gets the result.  `red`: T / 64 floats of LDS.
+template <int T>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = red[0];
 #pragma unroll
-  for (int i = 1; i < T / 64; ++i) v = f(v, red[i]);
+  for (int i = 1; i < T / 64; ++i) v += red[i];
   return v;
 }
 
-// exp2((z - m) c): m is at least z, or -inf where every z so far is
-__device__ __forceinline__ float weight_of(float z, float m, float c) {
-  return z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((z - m) * c);
+// exp2((z - m) c) for a finite m
+__device__ __forceinline__ float power(float z, float m, float c) { return __builtin_amdgcn_exp2f((z - m) * c); }
+// the same where m is -inf for every z being so
+__device__ __forceinline__ float weight_of(float z, float m, float c) { return m == -INFINITY ? 0.f : power(z, m, c); }
+
+// Joins the maxima and sums of T threads; every thread gets the row's.  `red`: T / 64 pairs of LDS.
+template <int T>
+__device__ __forceinline__ void join_threads(float& m, float& s, float c, float2* red) {
+  float top = wave_max(m);
+  s = wave_sum(s * weight_of(m, top, c));
+  m = top;
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(m, s);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) top = fmaxf(top, red[i].x);
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) s += red[i].y * weight_of(red[i].x, top, c);
+    m = top;
+  }
 }
 
-template <class E, int T>
-__global__ __launch_bounds__(T) void distill_kernel(DistillParams p) {
+// The teacher's side of a row, in LDS: per listed place its probability, the student's logit and the id, -1 for padding.
+struct Listed {
+  float* prob;
+  float* logit;
+  int* id;
+};
+constexpr int kRed = 32;         // floats of reductions in front of them
+inline int listed_lds(int k) { return (kRed + 3 * k) * 4; }
+
+// Every wave finds the teacher's maximum and sum for itself, the first one writes.  `any`: some probability is above zero.
+// The caller synchronises before it reads.
+template <class E>
+__device__ __forceinline__ Listed teach(float* lds, const DistillParams& p, long row, const E* z, float c, bool& any) {
+  const Listed l = {lds + kRed, lds + kRed + p.k, (int*)(lds + kRed + 2 * p.k)};
+  const int32_t* ids = p.ids + row * p.k;
+  const float* teacher = p.teacher + row * p.k;
+  const int lane = threadIdx.x & 63;
+  auto in = [&](int at) { return at >= 0 && at < p.vocab; };
+  float top = -INFINITY, sum = 0.f;
+  for (int k = lane; k < p.k; k += 64) {
+    const float t = teacher[k];
+    if (in(ids[k])) top = t > top || t != t ? t : top;
+  }
+  top = wave_max(top);
+  any = top != -INFINITY;
+  for (int k = lane; k < p.k; k += 64)
+    if (in(ids[k])) sum += weight_of(teacher[k], top, c);
+  sum = wave_sum(sum);
+  if (threadIdx.x < 64)
+    for (int k = lane; k < p.k; k += 64) {
+      const int at = ids[k];
+      l.id[k] = in(at) ? at : -1;
+      l.prob[k] = in(at) ? weight_of(teacher[k], top, c) / sum : 0.f;
+      l.logit[k] = in(at) ? load1(z + at) : -INFINITY;
+    }
+  return l;
+}
+
+// sum_k p_k (log p_k - (z_k - z_ref) / T) with z_ref, the largest of the logits that count: what the loss is short of is
+// log sum exp((z - z_ref) / T).  One wave.
+__device__ __forceinline__ float cross(const Listed& l, int n, float c, float& z_ref) {
+  const int lane = threadIdx.x & 63;
+  z_ref = -INFINITY;
+  for (int k = lane; k < n; k += 64)
+    if (!(l.prob[k] <= 0.f)) z_ref = fmaxf(z_ref, l.logit[k]);
+  z_ref = wave_max(z_ref);
+  if (z_ref == -INFINITY) z_ref = 0.f;      // all of them masked: the sum is infinite
+  float sum = 0.f;
+  for (int k = lane; k < n; k += 64) {
+    const float q = l.prob[k];
+    if (!(q <= 0.f)) sum += q * (log2f(q) - c * (l.logit[k] - z_ref));
+  }
+  return kLn2 * wave_sum(sum);
+}
+
+// A row from its first 16-byte boundary on: `head` elements before it, whole units, `tail` elements behind.
+template <class E>
+struct Span {
+  static constexpr int N = 16 / sizeof(E);
+  int head, units, tail;
+  __device__ __forceinline__ Span(const E* z, int vocab) {
+    head = min((int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(E), vocab);
+    units = (vocab - head) / N;
+    tail = vocab - head - units * N;
+  }
+  // the single element of a thread, -1: none
+  __device__ __forceinline__ int edge(int tid) const {
+    return tid < head ? tid : tid - head < tail ? head + units * N + tid - head : -1;
+  }
+};
+
+template <class E>
+__device__ __forceinline__ uint4 masked_unit() {
+  const uint32_t w = sizeof(E) == 2 ? 0xff80ff80u : 0xff800000u;     // -inf
+  return make_uint4(w, w, w, w);
+}
+template <class E>
+__device__ __forceinline__ float unit_max(const uint4& v, float m) {
+  float f[16 / sizeof(E)];
+  unpack<E>(v, f);
+#pragma unroll
+  for (int e = 0; e < 16 / (int)sizeof(E); ++e) m = fmaxf(m, f[e]);
+  return m;
+}
+template <class E>
+__device__ __forceinline__ float unit_sum(const uint4& v, float m, float c) {
+  float f[16 / sizeof(E)], s = 0.f;
+  unpack<E>(v, f);
+#pragma unroll
+  for (int e = 0; e < 16 / (int)sizeof(E); ++e) s += power(f[e], m, c);
+  return s;
+}
+// `together`: dz's units start where z's do
+template <class E, bool PAST>
+__device__ __forceinline__ void unit_grad(const uint4& v, float m, float c, float factor, E* dz, bool together) {
   constexpr int N = 16 / sizeof(E);
-  __shared__ float red[T / 64], prob[kMaxListed], listed[kMaxListed];
-  __shared__ int id[kMaxListed];
+  float f[N];
+  unpack<E>(v, f);
+#pragma unroll
+  for (int e = 0; e < N; ++e) f[e] = power(f[e], m, c) * factor;
+  if (together) {
+    const uint4 o = pack<E>(f);
+    if constexpr (PAST) {
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+      __builtin_nontemporal_store(u32x4{o.x, o.y, o.z, o.w}, (u32x4*)dz);
+    } else {
+      *(uint4*)dz = o;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) store1(dz + e, f[e]);
+  }
+}
+template <class E>
+__device__ __forceinline__ void zero_row(E* dz, int from, int to, int tid, int threads) {
+  constexpr int N = 16 / sizeof(E);
+  const Span<E> s(dz + from, to - from);
+  const int edge = s.edge(tid);
+  if (edge >= 0) store1(dz + from + edge, 0.f);
+  for (int u = tid; u < s.units; u += threads) *(uint4*)(dz + from + s.head + u * N) = make_uint4(0, 0, 0, 0);
+}
+
+// the listed places that are `mine`: the first of an id's entries writes for all of them
+template <class E, int T, class F>
+__device__ __forceinline__ void listed_grad(const Listed& l, int n, F&& mine, float m, float c, float factor,
+                                            float coef, E* dz) {
+  for (int k = threadIdx.x; k < n; k += T) {
+    const int at = l.id[k];
+    if (!mine(at)) continue;
+    float p = 0.f;
+    int first = n;
+#pragma unroll 8
+    for (int i = n - 1; i >= 0; --i) {
+      const bool same = l.id[i] == at;
+      p += same ? l.prob[i] : 0.f;
+      first = same ? i : first;
+    }
+    if (first == k) store1(dz + at, power(l.logit[k], m, c) * factor - coef * p);
+  }
+}
+
+// Maximum and sum of exponentials of this thread's part of a row: the edge element and its units, B at a time, of which
+// the first B stay in `held`.  Without a logit above -inf the maximum is -inf and the sum zero.
+template <class E, int T, int B>
+__device__ __forceinline__ void load_units(uint4 (&v)[B], const uint4* zu, int first, int units) {
+#pragma unroll
+  for (int i = 0; i < B; ++i) {
+    const int u = first + T * i;
+    v[i] = masked_unit<E>();
+    if (u < units) v[i] = zu[u];
+  }
+}
+template <class E, int T, int B>
+__device__ __forceinline__ void scan(const E* z, const uint4* zu, int edge, int units, float c, uint4 (&held)[B], float& m,
+                                     float& s) {
+  load_units<E, T, B>(held, zu, threadIdx.x, units);
+  m = edge >= 0 ? load1(z + edge) : -INFINITY;
+  if (m != m) {
+    s = m;               // NaN
+    m = -INFINITY;
+  } else {
+    s = m == -INFINITY ? 0.f : 1.f;
+  }
+  auto take = [&](const uint4 (&v)[B]) {
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < B; ++i) top = unit_max<E>(v[i], top);
+    const float at = top == -INFINITY ? 0.f : top;
+    s *= weight_of(m, top, c);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < B; ++i) s += unit_sum<E>(v[i], at, c);
+  };
+  take(held);
+  for (int u = threadIdx.x + T * B; u < units; u += T * B) {
+    uint4 v[B];
+    load_units<E, T, B>(v, zu, u, units);
+    take(v);
+  }
+}
+
+// WAVES: of a SIMD; PAST: the gradient is written past the caches, which then hold the logits for the second reading.
+template <class E, int T, int B, int WAVES, bool PAST>
+__global__ __launch_bounds__(T, WAVES) void distill_kernel(DistillParams p) {
+  constexpr int N = 16 / sizeof(E);
+  extern __shared__ float lds[];
   const int tid = threadIdx.x;
   const long row = blockIdx.x;
   const E* z = (const E*)p.z + row * p.ld;
   E* dz = p.dz ? (E*)p.dz + row * p.ldd : nullptr;
-  auto add = [](float a, float b) { return a + b; };
-  auto most = [](float a, float b) { return fmaxf(a, b); };
   const float w = p.weight ? p.weight[row] : 1.f;
   const float c = kLog2e / p.temperature;
-
-  // the teacher's side
-  float tmax = -INFINITY;
-  for (int k = tid; k < p.k; k += T) {
-    const int at = p.ids[row * p.k + k];
-    const bool in = at >= 0 && at < p.vocab;
-    const float t = in ? p.teacher[row * p.k + k] : -INFINITY;
-    id[k] = in ? at : -1;
-    prob[k] = t;
-    listed[k] = in ? load1(z + at) : 0.f;
-    tmax = t > tmax || t != t ? t : tmax;
-  }
-  tmax = reduce<T>(tmax, red, most);
-  float tsum = 0.f;
-  for (int k = tid; k < p.k; k += T) tsum += weight_of(prob[k], tmax, c);
-  tsum = reduce<T>(tsum, red, add);
-  bool live = w != 0.f && tmax != -INFINITY;
-
-  // the row from its first 16-byte boundary on: `head` elements before it, whole units, `tail` elements behind
-  const int head = min((int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(E), p.vocab);
-  const int units = (p.vocab - head) / N, tail = p.vocab - head - units * N;
-  const uint4* zu = (const uint4*)(z + head);
-  const int edge = tid < head ? tid : tid - head < tail ? head + units * N + tid - head : -1;   // this thread's single element
-
-  float m = -INFINITY, s = 0.f;
+  const Span<E> span(z, p.vocab);
+  const uint4* zu = (const uint4*)(z + span.head);
+  const int edge = span.edge(tid);
+  bool live = w != 0.f;
+  float m = 0.f, s = 0.f;
+  uint4 held[B];
+  Listed l = {};
   if (live) {
-    float ez = edge >= 0 ? load1(z + edge) : -INFINITY;
-    m = ez;
-    s = ez == -INFINITY ? 0.f : 1.f;
-    for (int u = tid; u < units; u += T) {
-      float f[N];
-      unpack<E>(zu[u], f);
-      float um = f[0];
-#pragma unroll
-      for (int e = 1; e < N; ++e) um = fmaxf(um, f[e]);
-      if (um > m) {
-        s *= weight_of(m, um, c);
-        m = um;
-      }
-#pragma unroll
-      for (int e = 0; e < N; ++e) s += weight_of(f[e], m, c);
-    }
-    const float all = reduce<T>(m, red, most);
-    s = reduce<T>(s * weight_of(m, all, c), red, add);
-    m = all;
-    live = m != -INFINITY;
+    bool any;
+    scan<E, T, B>(z, zu, edge, span.units, c, held, m, s);
+    l = teach(lds, p, row, z, c, any);
+    join_threads<T>(m, s, c, (float2*)lds);
+    live = any && !(m == -INFINITY && s == 0.f);      // (a row of NaN is not one without logits)
   }
   if (!live) {
     if (tid == 0) p.row_loss[row] = 0.f;
-    if (dz)
-      for (int i = tid; i < p.vocab; i += T) store1(dz + i, 0.f);
+    if (dz) zero_row(dz, 0, p.vocab, tid, T);
     return;
   }
-
-  float loss = 0.f;
-  for (int k = tid; k < p.k; k += T) {
-    const float pk = weight_of(prob[k], tmax, c) / tsum;
-    if (pk > 0.f || pk != pk) {
-      const float lp = kLn2 * (c * (prob[k] - tmax) - log2f(tsum));
-      loss += pk * (lp - kLn2 * (c * (listed[k] - m) - log2f(s)));
-    }
+  __syncthreads();       // the listed places are read, before any of the row is written
+  if (tid < 64) {
+    float z_ref;
+    const float own = cross(l, p.k, c, z_ref);
+    if (tid == 0) p.row_loss[row] = (own + kLn2 * (c * (m - z_ref) + log2f(s))) * (w * p.temperature * p.temperature);
   }
-  loss = reduce<T>(loss, red, add);
-  if (tid == 0) p.row_loss[row] = loss * (w * p.temperature * p.temperature);
   if (!dz) return;
-
-  const float coef = p.scale * w * p.temperature, part = coef / s;
+  const float coef = p.scale * w * p.temperature, factor = coef / s;
   const bool together = (((uintptr_t)dz - (uintptr_t)z) & 15) == 0;
-  if (edge >= 0) store1(dz + edge, weight_of(load1(z + edge), m, c) * part);
-  for (int u = tid; u < units; u += T) {
-    float f[N];
-    unpack<E>(zu[u], f);
+  if (edge >= 0) store1(dz + edge, power(load1(z + edge), m, c) * factor);
+  for (int first = tid; first < span.units; first += T * B) {
+    if (first != tid) load_units<E, T, B>(held, zu, first, span.units);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] = weight_of(f[e], m, c) * part;
-    if (together) {
-      ((uint4*)(dz + head))[u] = pack<E>(f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) store1(dz + head + u * N + e, f[e]);
+    for (int i = 0; i < B; ++i) {
+      const int u = first + T * i;
+      if (u < span.units) unit_grad<E, PAST>(held[i], m, c, factor, dz + span.head + (long)u * N, together);
     }
   }
   __syncthreads();
-  // the listed places: the first of an id's entries writes for all of them
-  for (int k = tid; k < p.k; k += T) {
-    if (id[k] < 0) continue;
-    float pk = 0.f;
-    bool first = true;
-    for (int i = 0; i < p.k; ++i)
-      if (id[i] == id[k]) {
-        first = first && i >= k;
-        pk += weight_of(prob[i], tmax, c) / tsum;
-      }
-    if (first) store1(dz + id[k], weight_of(listed[k], m, c) * part - coef * pk);
+  listed_grad<E, T>(l, p.k, [](int at) { return at >= 0; }, m, c, factor, coef, dz);
+}
+
+// ---------------------------------------------------------------------------
+// few rows, in pieces of whole units.  Workspace: 64 pairs of floats a row - the pieces' maxima and sums, and in
+// the last the listed part of the loss with its reference.
+// ---------------------------------------------------------------------------
+constexpr int kPieceThreads = 256, kPieceHeld = 8;
+constexpr int kPieces = 62, kPieceRows = 256;
+
+template <class E>
+__global__ __launch_bounds__(kPieceThreads) void distill_scan_kernel(DistillParams p, float2* ws, int per) {
+  constexpr int T = kPieceThreads;
+  extern __shared__ float lds[];
+  const long row = blockIdx.y;
+  const E* z = (const E*)p.z + row * p.ld;
+  const float w = p.weight ? p.weight[row] : 1.f, c = kLog2e / p.temperature;
+  const Span<E> span(z, p.vocab);
+  if (blockIdx.x + 1 == gridDim.x) {       // the listed places, beside the pieces
+    if (threadIdx.x >= 64) return;
+    float z_ref = 0.f, own = 0.f;
+    bool any = false;
+    if (w != 0.f) {
+      const Listed l = teach(lds, p, row, z, c, any);
+      if (any) own = cross(l, p.k, c, z_ref);
+    }
+    if (threadIdx.x == 0) ws[row * 64 + 63] = any ? make_float2(own, z_ref) : make_float2(0.f, -INFINITY);   // (-inf: nothing listed)
+    return;
   }
+  const int first = blockIdx.x * per, units = max(min(per, span.units - first), 0);
+  float m = -INFINITY, s = 0.f;
+  if (w != 0.f) {
+    uint4 held[kPieceHeld];
+    scan<E, T, kPieceHeld>(z, (const uint4*)(z + span.head) + first, blockIdx.x ? -1 : span.edge(threadIdx.x), units, c, held, m, s);
+    join_threads<T>(m, s, c, (float2*)lds);
+  }
+  if (threadIdx.x == 0) ws[row * 64 + blockIdx.x] = make_float2(m, s);
+}
+
+// a row's maximum and sum from its pieces
+__device__ __forceinline__ void join(const float2* ws, int pieces, float c, float& m, float& s) {
+  m = -INFINITY;
+  s = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < pieces; ++i) {
+    const float2 v = ws[i];
+    const float top = fmaxf(m, v.x);
+    s = s * weight_of(m, top, c) + v.y * weight_of(v.x, top, c);
+    m = top;
+  }
+}
+
+// The last blockIdx.y: the losses; the others a row each, of which a workgroup writes the gradient of one piece.
+template <class E>
+__global__ __launch_bounds__(kPieceThreads) void distill_grad_kernel(DistillParams p, const float2* ws, int pieces, int per,
+                                                                     int rows, float* loss) {
+  constexpr int T = kPieceThreads, N = 16 / sizeof(E);
+  extern __shared__ float lds[];
+  const int tid = threadIdx.x;
+  const float c = kLog2e / p.temperature;
+  if (blockIdx.y + 1 == gridDim.y) {
+    if (blockIdx.x) return;
+    float sum = 0.f;
+    if (tid < rows) {                 // fewer than T
+      const float w = p.weight ? p.weight[tid] : 1.f;
+      const float2 own = ws[tid * 64 + 63];
+      float m, s;
+      join(ws + tid * 64, pieces, c, m, s);
+      if (w != 0.f && own.y != -INFINITY && !(m == -INFINITY && s == 0.f))
+        sum = (own.x + kLn2 * (c * (m - own.y) + log2f(s))) * (w * p.temperature * p.temperature);
+      p.row_loss[tid] = sum;
+    }
+    sum = block_sum<T>(sum, lds);
+    if (tid == 0 && loss) *loss = sum * p.scale;
+    return;
+  }
+  const long row = blockIdx.y;
+  const E* z = (const E*)p.z + row * p.ld;
+  E* dz = (E*)p.dz + row * p.ldd;
+  const float w = p.weight ? p.weight[row] : 1.f;
+  const Span<E> span(z, p.vocab);
+  const int first = blockIdx.x * per, units = max(min(per, span.units - first), 0);
+  const int from = span.head + first * N, to = from + units * N;
+  const int edge = blockIdx.x ? -1 : span.edge(tid);
+  const uint4* zu = (const uint4*)(z + from);
+  uint4 held[kPieceHeld];
+  load_units<E, T, kPieceHeld>(held, zu, tid, units);
+  // (everything a workgroup waits for is under way before it looks at any of it)
+  const int lane = tid & 63;
+  const float2 piece = lane < pieces ? ws[row * 64 + lane] : make_float2(-INFINITY, 0.f);
+  const float none = ws[row * 64 + 63].y;
+  bool any;
+  const Listed l = teach(lds, p, row, z, c, any);
+  const float m = wave_max(piece.x), s = wave_sum(piece.y * weight_of(piece.x, m, c));
+  __syncthreads();       // the listed places are read, before any of the row is written
+  if (w == 0.f || (m == -INFINITY && s == 0.f) || none == -INFINITY) {
+    if (edge >= 0) store1(dz + edge, 0.f);
+    zero_row(dz, from, to, tid, T);
+    return;
+  }
+  const float coef = p.scale * w * p.temperature, factor = coef / s;
+  const bool together = (((uintptr_t)dz - (uintptr_t)z) & 15) == 0;
+  if (edge >= 0) store1(dz + edge, power(load1(z + edge), m, c) * factor);
+  for (int at = tid; at < units; at += T * kPieceHeld) {
+    if (at != tid) load_units<E, T, kPieceHeld>(held, zu, at, units);
+#pragma unroll
+    for (int i = 0; i < kPieceHeld; ++i)
+      if (at + T * i < units) unit_grad<E, false>(held[i], m, c, factor, dz + from + (long)(at + T * i) * N, together);
+  }
+  __syncthreads();
+  // (the row's edges are the first piece's)
+  listed_grad<E, T>(l, p.k, [&](int at) {
+    return (at >= from && at < to) || (blockIdx.x == 0 && at >= 0 && (at < span.head || at >= span.head + span.units * N));
+  }, m, c, factor, coef, dz);
 }
 
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* row_loss, long rows, float scale, float* loss) {
   __shared__ float red[16];
   float s = 0.f;
   for (long i = threadIdx.x; i < rows; i += 1024) s += row_loss[i];
-  s = reduce<1024>(s, red, [](float a, float b) { return a + b; });
+  s = block_sum<1024>(s, red);
   if (threadIdx.x == 0) *loss = s * scale;
 }
 
+// By the units of 16 bytes in a row.  More threads a row, so fewer rows at a time, as rows get longer: the rows being worked
+// on, 2048 threads of them on a CU or half as many, stay in the 256 MB of cache in front of the memory until they are
+// read again.  bf16 rows need all the waves for their exponentials (4096 x 128256: 445 us with 4 units and 8 waves
+// a SIMD, 492 with 8 and 4), f32 rows, half as many of them a byte, more loads per wave (2048 x 128256: 451 and 419), as
+// do rows that 256 threads take in two trips (16384 x 32000 bf16: 445 and 409).  Rows of at most 8 KB are a wave's, written
+// through the caches (65536 x 2000: 128 us, past them 142; 4096 x 128256: 479 and 445, f32 2048 x 128256: 633 and 451).
 template <class E>
 void launch(hipStream_t st, const DistillParams& p, long rows) {
-  if (p.vocab <= 8192)
-    hipLaunchKernelGGL((distill_kernel<E, 256>), dim3((unsigned)rows), dim3(256), 0, st, p);
-  else
-    hipLaunchKernelGGL((distill_kernel<E, 1024>), dim3((unsigned)rows), dim3(1024), 0, st, p);
+  const int units = p.vocab / (16 / (int)sizeof(E));
+#define JPP_D(T_, B_, W_, P_)                                                                                           \
+  hipLaunchKernelGGL((distill_kernel<E, T_, B_, W_, P_>), dim3((unsigned)rows), dim3(T_), listed_lds(p.k), st, p)
+  constexpr int B = sizeof(E) == 2 ? 4 : 8, W = sizeof(E) == 2 ? 8 : 4;
+  if (units <= 512) JPP_D(64, 4, 8, false);
+  else if (units <= 2048) JPP_D(256, 4, 8, true);
+  else if (units <= 4096) JPP_D(256, 8, 4, true);
+  else if (units <= 8192) JPP_D(512, B, W, true);
+  else JPP_D(1024, B, W, true);
+#undef JPP_D
+}
+
+template <class E>
+int launch_pieces(hipStream_t st, const DistillParams& p, int rows, float* loss, float2* ws, int pieces, int per) {
+  hipLaunchKernelGGL((distill_scan_kernel<E>), dim3(pieces + 1, rows), dim3(kPieceThreads), listed_lds(p.k), st, p, ws, per);
+  JPP_LAUNCH_CHECK();
+  // (without a gradient only the losses' workgroup)
+  hipLaunchKernelGGL((distill_grad_kernel<E>), dim3(p.dz ? pieces : 1, p.dz ? rows + 1 : 1), dim3(kPieceThreads), listed_lds(p.k), st,
+                     p, ws, pieces, per, rows, loss);
+  JPP_LAUNCH_CHECK();
+  return JPP_OK;
 }
 
 }  // namespace
@@ -216,12 +504,19 @@ extern "C" int jpp_distill_loss(void* stream, const jpp_distill_args* a) {
   JPP_REQUIRE(a->logits && a->ids && a->teacher && a->row_loss, "%s: null operand", who);
   JPP_REQUIRE(a->ld >= a->vocab && (!a->dlogits || a->ldd >= a->vocab), "%s: leading dimension too small", who);
   JPP_REQUIRE(((uintptr_t)a->logits | (uintptr_t)a->dlogits) % 16 == 0, "%s: logits and dlogits must be 16-byte aligned", who);
+  JPP_REQUIRE((uintptr_t)a->workspace % 8 == 0, "%s: workspace must be 8-byte aligned", who);
   JPP_REQUIRE(a->dlogits != a->logits || a->ldd == a->ld, "%s: dlogits over logits with another leading dimension", who);
   DistillParams p = {a->logits, a->ids, a->teacher, a->weight, a->row_loss, a->dlogits, (long)a->ld, (long)a->ldd,
                      (int)a->vocab, a->k, a->temperature, a->scale};
   const double n = (double)a->rows * a->vocab, es = a->dtype == JPP_DTYPE_F32 ? 4 : 2;
   ProbeScope probe(st, "distill_loss", 0, es * n * (a->dlogits ? 2 : 1));
-  if (a->dtype == JPP_DTYPE_F32) launch<float>(st, p, a->rows);
+  const bool f32 = a->dtype == JPP_DTYPE_F32;
+  const int units = (int)(a->vocab / (f32 ? 4 : 8));
+  const int per = std::max(kPieceThreads * kPieceHeld, (units + kPieces - 1) / kPieces), pieces = (units + per - 1) / per;
+  if (a->workspace && a->rows < kPieceRows && pieces > 1)
+    return f32 ? launch_pieces<float>(st, p, (int)a->rows, a->loss, (float2*)a->workspace, pieces, per)
+               : launch_pieces<bf16_t>(st, p, (int)a->rows, a->loss, (float2*)a->workspace, pieces, per);
+  if (f32) launch<float>(st, p, a->rows);
   else launch<bf16_t>(st, p, a->rows);
   JPP_LAUNCH_CHECK();
   if (a->loss) {
