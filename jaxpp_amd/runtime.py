@@ -662,58 +662,51 @@ def linattn_workspace(batch, seq, n_heads, n_kv_heads, head_dim, backward=False,
 def linattn_fwd(q, k, v, o, decay, ldq, ldk, ldv, ldo, batch, seq, n_heads, n_kv_heads, head_dim, scale, state_in=None,
                 state_out=None, lens=None, workspace=None, f32=False, stream=None):
     """Linear attention with a decay for each head (jpp_linattn_fwd)."""
-    a = LinattnArgs(q=q, k=k, v=v, o=o, decay=decay, state_in=state_in, state_out=state_out, lens=lens,
-                    workspace=workspace, ldq=ldq, ldk=ldk, ldv=ldv, ldo=ldo, batch=batch, seq=seq, n_heads=n_heads,
-                    n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale, dtype=int(f32))
-    check(load().jpp_linattn_fwd(stream, C.byref(a)))
+    check(load().jpp_linattn_fwd(stream, LinattnArgs(
+        q, k, v, o, None, None, None, None, decay, state_in, state_out, None, None, lens, workspace, ldq, ldk, ldv, ldo,
+        0, 0, 0, 0, batch, seq, n_heads, n_kv_heads, head_dim, scale, f32)))
 
 
 def linattn_bwd(q, k, v, d_o, dq, dk, dv, decay, ldq, ldk, ldv, lddo, lddq, lddk, lddv, batch, seq, n_heads, n_kv_heads,
                 head_dim, scale, state_in=None, d_state_out=None, d_state_in=None, lens=None, workspace=None, f32=False,
                 stream=None):
     """Its gradients (jpp_linattn_bwd)."""
-    a = LinattnArgs(q=q, k=k, v=v, d_o=d_o, dq=dq, dk=dk, dv=dv, decay=decay, state_in=state_in,
-                    d_state_out=d_state_out, d_state_in=d_state_in, lens=lens, workspace=workspace, ldq=ldq, ldk=ldk,
-                    ldv=ldv, lddo=lddo, lddq=lddq, lddk=lddk, lddv=lddv, batch=batch, seq=seq, n_heads=n_heads,
-                    n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale, dtype=int(f32))
-    check(load().jpp_linattn_bwd(stream, C.byref(a)))
+    check(load().jpp_linattn_bwd(stream, LinattnArgs(
+        q, k, v, None, d_o, dq, dk, dv, decay, state_in, None, d_state_out, d_state_in, lens, workspace, ldq, ldk, ldv, 0,
+        lddo, lddq, lddk, lddv, batch, seq, n_heads, n_kv_heads, head_dim, scale, f32)))
 
 
 def linattn_step(q, k, v, o, decay, state_in, state_out, ldq, ldk, ldv, ldo, batch, n_heads, n_kv_heads, head_dim, scale,
                  f32=False, stream=None):
     """One token per sequence (jpp_linattn_step); `state_out` may be `state_in`."""
-    a = LinattnArgs(q=q, k=k, v=v, o=o, decay=decay, state_in=state_in, state_out=state_out, ldq=ldq, ldk=ldk, ldv=ldv,
-                    ldo=ldo, batch=batch, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, scale=scale,
-                    dtype=int(f32))
-    check(load().jpp_linattn_step(stream, C.byref(a)))
+    check(load().jpp_linattn_step(stream, LinattnArgs(
+        q, k, v, o, None, None, None, None, decay, state_in, state_out, None, None, None, None, ldq, ldk, ldv, ldo,
+        0, 0, 0, 0, batch, 0, n_heads, n_kv_heads, head_dim, scale, f32)))
 
 
 def block_join_fwd(x, b, h, rows, cols, y=None, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None, rstd_post=None,
                    rstd_pre=None, alpha=1.0, eps=1e-6, f32=False, stream=None):
     """A block's output joined to the residual stream: norm, gate, residual scale, next norm (jpp_block_join_fwd)."""
-    a = JoinArgs(x=x, b=b, gamma_post=gamma_post, gate=gate, gamma_pre=gamma_pre, h=h, y=y, rstd_post=rstd_post,
-                 rstd_pre=rstd_pre, rows=rows, cols=cols, gate_rows=gate_rows, alpha=alpha, eps=eps, dtype=int(f32))
-    check(load().jpp_block_join_fwd(stream, C.byref(a)))
+    check(load().jpp_block_join_fwd(stream, JoinArgs(
+        x, b, gamma_post, gate, gamma_pre, h, y, rstd_post, rstd_pre, None, None, None, None, None, None, None, None, rows,
+        cols, gate_rows, alpha, eps, 0, f32)))
 
 
 def block_join_bwd(h, b, dh, dy, dx, db, rows, cols, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None,
                    rstd_post=None, rstd_pre=None, dgamma_post=None, dgate=None, dgamma_pre=None, workspace=None,
                    alpha=1.0, accumulate=True, f32=False, stream=None):
     """Its gradients (jpp_block_join_bwd); the sums over rows are added to what is there if `accumulate`."""
-    a = JoinArgs(b=b, gamma_post=gamma_post, gate=gate, gamma_pre=gamma_pre, h=h, rstd_post=rstd_post, rstd_pre=rstd_pre,
-                 dh=dh, dy=dy, dx=dx, db=db, dgamma_post=dgamma_post, dgate=dgate, dgamma_pre=dgamma_pre,
-                 workspace=workspace, rows=rows, cols=cols, gate_rows=gate_rows, alpha=alpha, accumulate=int(accumulate),
-                 dtype=int(f32))
-    check(load().jpp_block_join_bwd(stream, C.byref(a)))
+    check(load().jpp_block_join_bwd(stream, JoinArgs(
+        None, b, gamma_post, gate, gamma_pre, h, None, rstd_post, rstd_pre, dh, dy, dx, db, dgamma_post, dgate, dgamma_pre,
+        workspace, rows, cols, gate_rows, alpha, 0.0, accumulate, f32)))
 
 
 def distill_loss(logits, ids, teacher, rows, vocab, k, ld, row_loss, loss=None, dlogits=None, ldd=0, weight=None,
                  temperature=1.0, scale=1.0, workspace=None, f32=False, stream=None):
     """Loss and gradient of logits against a teacher's top logits (jpp_distill_loss)."""
-    a = DistillArgs(logits=logits, ids=ids, teacher=teacher, weight=weight, row_loss=row_loss, loss=loss,
-                    dlogits=dlogits, workspace=workspace, ld=ld, ldd=ldd, rows=rows, vocab=vocab, k=k, temperature=temperature, scale=scale,
-                    dtype=int(f32))
-    check(load().jpp_distill_loss(stream, C.byref(a)))
+    check(load().jpp_distill_loss(stream, DistillArgs(
+        logits, ids, teacher, weight, row_loss, loss, dlogits, workspace, ld, ldd, rows, vocab, k, temperature, scale,
+        f32)))
 
 
 # Elements of tensors that travel in one call, or one larger tensor (of a layer's results, the layer): what bounds the
