@@ -15,11 +15,11 @@
 //
 // so one pair of kernels, given the tensors by a "role", computes all of them.
 //
-// A workgroup walks a segment of a sequence in chunks of rows (bf16: 64): within a chunk the pairs
-// are products of tiles, between chunks the state is carried in f32 accumulators, each wave 32
-// of its columns.  Where batch x heads give too few workgroups, a sequence is cut into segments:
-// a first launch sums every segment's y^T z, a second carries them over the segments (small), and the
-// walk starts each segment from its state.
+// A workgroup walks a segment of a sequence in chunks of rows (bf16: 64, f32: 32): within a chunk the pairs
+// are products of tiles, between chunks the state is carried in f32 accumulators, each wave some columns of it.
+// Where batch x heads give too few workgroups, a sequence is cut into segments: a first launch sums
+// every segment's y^T z, a second carries them over the segments (small), and the walk starts each segment from
+// its state.
 #include <math.h>
 
 #include <algorithm>
@@ -55,7 +55,7 @@ struct Params {
   int n_roles, n_sums;           // of which the first n_sums own their `parts`
   const float* decay;
   const int32_t* lens;
-  int batch, seq, heads, n_seg, seg_rows;
+  int batch, seq, heads, group, n_seg, seg_rows;   // group: query heads per key head
 };
 
 struct Place {
@@ -77,17 +77,24 @@ __device__ __forceinline__ int rows_of(const Params& p, int b) {
   return p.lens ? min(max(p.lens[b], 0), p.seq) : p.seq;
 }
 
-// Workgroups of one (segment, batch) follow each other over the heads, and the roles over those: what
-// they share is read at about the same time.
+// Workgroups are dealt to the 8 XCDs in turn, each of which has an L2 of its own.  The roles and the query heads that
+// read the same rows of the same heads - n_roles x group workgroups - go to one XCD, one after the other, where their number
+// allows it.
 __device__ __forceinline__ Place place(const Params& p, int n_roles) {
   Place w;
-  unsigned i = blockIdx.x;
-  w.role = i % n_roles;
-  i /= n_roles;
-  w.h = i % p.heads;
-  i /= p.heads;
-  w.seg = i % p.n_seg;
-  w.b = i / p.n_seg;
+  const unsigned shared = n_roles * p.group, sets = gridDim.x / shared;
+  unsigned set = blockIdx.x / shared, member = blockIdx.x % shared;
+  if ((sets & 7) == 0) {
+    const unsigned turn = blockIdx.x >> 3;
+    set = (turn / shared) * 8 + (blockIdx.x & 7);
+    member = turn % shared;
+  }
+  const unsigned kv = p.heads / p.group;
+  w.role = member % n_roles;
+  w.h = (set % kv) * p.group + member / n_roles;
+  set /= kv;
+  w.seg = set % p.n_seg;
+  w.b = set / p.n_seg;
   w.s0 = w.seg * p.seg_rows;
   w.s1 = min(w.s0 + p.seg_rows, p.seq);
   w.live = min(max(rows_of(p, w.b) - w.s0, 0), w.s1 - w.s0);
@@ -112,14 +119,6 @@ __device__ __forceinline__ bf16x8 split(float (&v)[8]) {
 __device__ __forceinline__ bf16x8 nearest(const float (&v)[8]) {
   return __builtin_bit_cast(bf16x8, make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])));
 }
-__device__ __forceinline__ void acc8(float (&v)[8], const f32x16& a, int base) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = a[base + e];
-}
-__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
 // LDS by byte addresses, so that tiles, slabs and row blocks are offsets of the instruction
 template <class V> __device__ __forceinline__ V lds_get(uint32_t at) {
   return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
@@ -136,15 +135,14 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // ---------------------------------------------------------------------------
 template <int D>
 struct Tile {
-  static constexpr int THREADS = 2 * D;              // D / 32 waves
+  static constexpr int THREADS = 256;
   static constexpr int BYTES = kChunk * D * 2;
   static constexpr int UNITS = D / 8;                // 16-byte units of a row
   static constexpr int PER = kChunk * UNITS / THREADS;
-  static_assert(PER == 4 && THREADS / UNITS == 16, "a thread has a unit of every 16th row");
+  static constexpr int STEP = THREADS / UNITS;       // a thread has a unit of every STEP-th row, 16 or 32: the same swizzle
   typedef u32x4 Regs[PER];
 
-  // the thread's byte offset from a chunk's first row, and its place in a tile (rows 16 apart have the
-  // same swizzle)
+  // the thread's byte offset from a chunk's first row, and its place in a tile
   static __device__ __forceinline__ uint32_t offset(long ld) {
     return (uint32_t)((threadIdx.x / UNITS) * ld + (threadIdx.x % UNITS) * 8) * 2;
   }
@@ -156,35 +154,159 @@ struct Tile {
     const uint8_t* base = (const uint8_t*)src;
     if (live >= kChunk) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) r[i] = *(const u32x4*)(base + 32 * i * ld + off);
+      for (int i = 0; i < PER; ++i) r[i] = *(const u32x4*)(base + 2 * STEP * i * ld + off);
     } else {
       const int row = threadIdx.x / UNITS;
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        r[i] = row + 16 * i < live ? *(const u32x4*)(base + 32 * i * ld + off) : u32x4{0, 0, 0, 0};
+      for (int i = 0; i < PER; ++i) {
+        r[i] = u32x4{0, 0, 0, 0};
+        if (row + STEP * i < live) r[i] = *(const u32x4*)(base + 2 * STEP * i * ld + off);
+      }
     }
   }
   static __device__ __forceinline__ void put(uint32_t at, const Regs& r) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) lds_put(at + i * 2048, r[i]);
+    for (int i = 0; i < PER; ++i) lds_put(at + i * STEP * 128, r[i]);
   }
 };
 
-// Operand whose rows are a tile's columns 32 t .. + 31 and whose contraction runs over the tile's rows 16 st .. + 15 in the
-// accumulators' order (as slab_frag_tr): `at` = the tile's address + tr_base(lane).
-__device__ __forceinline__ uint32_t tr_base(int lane) {
-  const int g = lane >> 4, s = lane & 15;
-  const int k = ((g >> 1) << 2) + (s >> 2), n = ((g & 1) << 4) + ((s & 3) << 2);
-  return slab_off(k, n >> 3) + ((n & 7) << 1);
+// Two layouts of the same walk, both with four waves a workgroup: heads of 128 on 32 x 32 accumulators, a wave 32 columns
+// of the state; heads of 64 on 16 x 16 ones, a wave 16 columns.  (Heads of 128 on eight waves of 16 columns read their
+// operands from LDS twice as often: gradients of 2 x 4096 x 32 heads 334 us, 276 like this; heads of 64 on two waves
+// of 32 columns leave one or two waves on a SIMD: 116 us, 106 like this.)
+//
+// An accumulator holds column lane % W and, in register r, row 8 (r / 4) + 4 h + r % 4 (W = 32, h = lane / 32) or 4 g + r
+// (W = 16, g = lane / 16).  Eight registers - half of one accumulator, or two that lie one below the other - are an
+// operand whose contraction runs over 16 or 32 rows in that order, "the accumulators' order".  Operands
+// from LDS that meet one are read in it.
+template <int W> struct Layout;
+
+template <>
+struct Layout<32> {
+  typedef f32x16 Acc;
+  static constexpr int K = 16;                       // contraction of one MFMA
+  static __device__ __forceinline__ Acc mfma(const bf16x8& a, const bf16x8& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int line(int lane) { return lane & 31; }
+  static __device__ __forceinline__ int row_of(int lane, int r) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
+  // step k of a contraction over accumulators' rows
+  template <int N>
+  static __device__ __forceinline__ void take(float (&v)[8], const Acc (&a)[N], int k) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = a[k >> 1][(k & 1) * 8 + e];
+  }
+  // LDS addresses within a slab, for this lane: `row` its row of a block of W, swizzled
+  static __device__ __forceinline__ uint32_t row(int lane) { return slab_off(lane & 31, 0); }
+  static __device__ __forceinline__ uint32_t step(uint32_t row, int lane, int k) {       // rows' elements K k .. in memory order
+    return (row ^ ((k & 3) * 32 + (lane >> 5) * 16)) + (k >> 2) * 8192;
+  }
+  static __device__ __forceinline__ bf16x8 ordered(uint32_t tile, uint32_t row, int lane, int k) {   // and in the accumulators' order
+    const uint32_t at = tile + (k >> 2) * 8192 + (lane >> 5) * 8;
+    const u32x2 a = lds_get<u32x2>(at + (row ^ ((k & 3) * 32))), b = lds_get<u32x2>(at + (row ^ ((k & 3) * 32 + 16)));
+    return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+  }
+  // operand whose rows are a tile's columns 32 t .. and whose contraction runs over its rows 16 k .., in the accumulators' order;
+  // `at` = the tile's address + tr(lane)
+  static __device__ __forceinline__ uint32_t tr(int lane) {
+    const int g = lane >> 4, s = lane & 15;
+    const int k = ((g >> 1) << 2) + (s >> 2), n = ((g & 1) << 4) + ((s & 3) << 2);
+    return slab_off(k, n >> 3) + ((n & 7) << 1);
+  }
+  static __device__ __forceinline__ bf16x8 columns(uint32_t at, int t, int k) {
+    typedef __attribute__((address_space(3))) s16x4* p16;
+    // 8 rows, like 32 columns, flip bit 2 of the 16-byte unit
+    const uint32_t from = (at ^ ((t & 1) << 6)) + (t >> 1) * 8192 + k * 2048;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)from);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)((from ^ 64) + 1024));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // per-row weights of a contraction step
+  static __device__ __forceinline__ void weights(f32x4 (&w)[2], uint32_t table, int lane, int k) {
+    w[0] = lds_get<f32x4>(table + (lane >> 5) * 16 + k * 64);
+    w[1] = lds_get<f32x4>(table + (lane >> 5) * 16 + k * 64 + 32);
+  }
+  // a tile of pairs, rows j (accumulator) by i, as operand units of row i, in two parts
+  static __device__ __forceinline__ void put_pairs(uint32_t at, uint32_t row, int lane, int jt, const Acc& s);
+  // four neighbouring columns of a row of the result: register group q of a wave's columns
+  static constexpr int GROUPS = 4;
+  static __device__ __forceinline__ uint32_t out(uint32_t row, int lane, int wave, int q) {
+    return (wave >> 1) * 8192 + (row ^ ((wave & 1) * 64 + q * 16)) + (lane >> 5) * 8;
+  }
+  static __device__ __forceinline__ int out_col(int lane, int q) { return q * 8 + (lane >> 5) * 4; }
+};
+
+template <>
+struct Layout<16> {
+  typedef f32x4 Acc;
+  static constexpr int K = 32;
+  static __device__ __forceinline__ Acc mfma(const bf16x8& a, const bf16x8& b, const Acc& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int line(int lane) { return lane & 15; }
+  static __device__ __forceinline__ int row_of(int lane, int r) { return (lane >> 4) * 4 + r; }
+  template <int N>
+  static __device__ __forceinline__ void take(float (&v)[8], const Acc (&a)[N], int k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[2 * k][e];
+      v[4 + e] = a[2 * k + 1][e];
+    }
+  }
+  static __device__ __forceinline__ uint32_t row(int lane) { return slab_off(lane & 15, 0); }
+  static __device__ __forceinline__ uint32_t step(uint32_t row, int lane, int k) {
+    return (row ^ ((k & 1) * 64 + (lane >> 4) * 16)) + (k >> 1) * 8192;
+  }
+  static __device__ __forceinline__ bf16x8 ordered(uint32_t tile, uint32_t row, int lane, int k) {
+    // elements 4 g .. + 3 are half of unit g / 2, 16 + 4 g .. of the next but one
+    const uint32_t at = tile + (k >> 1) * 8192 + ((lane >> 4) & 1) * 8, unit = row ^ ((k & 1) * 64 + (lane >> 5) * 16);
+    const u32x2 a = lds_get<u32x2>(at + unit), b = lds_get<u32x2>(at + (unit ^ 32));
+    return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+  }
+  static __device__ __forceinline__ uint32_t tr(int lane) {
+    const int s = lane & 15, n = (s & 3) << 2;
+    return slab_off((lane >> 4) * 4 + (s >> 2), n >> 3) + ((n & 7) << 1);
+  }
+  static __device__ __forceinline__ bf16x8 columns(uint32_t at, int t, int k) {
+    typedef __attribute__((address_space(3))) s16x4* p16;
+    const uint32_t from = (at ^ ((t & 3) << 5)) + (t >> 2) * 8192 + k * 4096;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)from);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)(from + 2048));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  static __device__ __forceinline__ void weights(f32x4 (&w)[2], uint32_t table, int lane, int k) {
+    w[0] = lds_get<f32x4>(table + (lane >> 4) * 16 + k * 128);
+    w[1] = lds_get<f32x4>(table + (lane >> 4) * 16 + k * 128 + 64);
+  }
+  static __device__ __forceinline__ void put_pairs(uint32_t at, uint32_t row, int lane, int jt, const Acc& s);
+  static constexpr int GROUPS = 1;
+  static __device__ __forceinline__ uint32_t out(uint32_t row, int lane, int wave, int q) {
+    return (wave >> 2) * 8192 + (row ^ ((wave & 3) * 32 + (lane >> 5) * 16)) + ((lane >> 4) & 1) * 8;
+  }
+  static __device__ __forceinline__ int out_col(int lane, int q) { return (lane >> 4) * 4; }
+};
+
+__device__ __forceinline__ void Layout<32>::put_pairs(uint32_t at, uint32_t row, int lane, int jt, const Acc& s) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = s[k * 8 + e];
+    const uint32_t to = at + step(row, lane, jt * 2 + k);
+    lds_put(to, split(v));
+    lds_put(to + 8192, nearest(v));
+  }
 }
-__device__ __forceinline__ bf16x8 tr_frag(uint32_t at, int t, int st) {
-  // 8 rows, like 32 columns, flip bit 2 of the 16-byte unit
-  const uint32_t even = at + (t >> 1) * 8192 + st * 2048, odd = (at ^ 64) + (t >> 1) * 8192 + st * 2048;
-  typedef __attribute__((address_space(3))) s16x4* p16;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)(t & 1 ? odd : even));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)((t & 1 ? even : odd) + 1024));
-  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+__device__ __forceinline__ void Layout<16>::put_pairs(uint32_t at, uint32_t row, int lane, int jt, const Acc& s) {
+  const uint32_t to = at + (row ^ ((jt >> 1) * 64 + (lane >> 4) * 16)) + (jt & 1) * 8;
+  const u32x2 hi = {pack2(s[0], s[1]), pack2(s[2], s[3])};
+  lds_put(to, hi);
+  lds_put(to + 8192, u32x2{pack2(s[0] - bf16lo_to_f32(hi.x), s[1] - bf16hi_to_f32(hi.x)),
+                           pack2(s[2] - bf16lo_to_f32(hi.y), s[3] - bf16hi_to_f32(hi.y))});
 }
+// the layout of heads of D
+template <int D>
+using LayoutOf = Layout<D / 4>;
 
 // A head's decay by distances, in LDS: of pairs (i - j + 64, zero on the side that does not count), and of the
 // chunk's rows in the state's update and in what they take from it.
@@ -208,55 +330,60 @@ __device__ __forceinline__ void row_weights(Weights* w, float g2, float a_update
 // S += y^T (w z): z as operand times its rows' weights in PARTS bf16 - three hold all 24 bits of the
 // products, for a state that is a result; two, 16 bits, for one that only meets x as two bf16.
 template <int D, int PARTS>
-__device__ __forceinline__ void update_state(f32x16 (&S)[D / 32], uint32_t ytr, const bf16x8 (&zf)[4], uint32_t up,
-                                             int lane) {
+__device__ __forceinline__ void update_state(typename LayoutOf<D>::Acc (&S)[4], uint32_t ytr,
+                                             const bf16x8 (&zf)[kChunk / LayoutOf<D>::K], uint32_t up, int lane) {
+  using L = LayoutOf<D>;
 #pragma unroll
-  for (int st = 0; st < 4; ++st) {
-    const u32x4 zw = __builtin_bit_cast(u32x4, zf[st]);
-    const f32x4 w0 = lds_get<f32x4>(up + (lane >> 5) * 16 + st * 64);
-    const f32x4 w1 = lds_get<f32x4>(up + (lane >> 5) * 16 + st * 64 + 32);
-    float z[8] = {bf16lo_to_f32(zw.x) * w0.x, bf16hi_to_f32(zw.x) * w0.y, bf16lo_to_f32(zw.y) * w0.z,
-                  bf16hi_to_f32(zw.y) * w0.w, bf16lo_to_f32(zw.z) * w1.x, bf16hi_to_f32(zw.z) * w1.y,
-                  bf16lo_to_f32(zw.w) * w1.z, bf16hi_to_f32(zw.w) * w1.w};
+  for (int k = 0; k < kChunk / L::K; ++k) {
+    const u32x4 zw = __builtin_bit_cast(u32x4, zf[k]);
+    f32x4 w[2];
+    L::weights(w, up, lane, k);
+    float z[8] = {bf16lo_to_f32(zw.x) * w[0].x, bf16hi_to_f32(zw.x) * w[0].y, bf16lo_to_f32(zw.y) * w[0].z,
+                  bf16hi_to_f32(zw.y) * w[0].w, bf16lo_to_f32(zw.z) * w[1].x, bf16hi_to_f32(zw.z) * w[1].y,
+                  bf16lo_to_f32(zw.w) * w[1].z, bf16hi_to_f32(zw.w) * w[1].w};
     bf16x8 part[PARTS];
 #pragma unroll
     for (int i = 0; i + 1 < PARTS; ++i) part[i] = split(z);
     part[PARTS - 1] = nearest(z);
-    bf16x8 yf[D / 32];
+    bf16x8 yf[4];
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t) yf[t] = tr_frag(ytr, t, st);
+    for (int t = 0; t < 4; ++t) yf[t] = L::columns(ytr, t, k);
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i)
+    for (int i = 0; i < PARTS; ++i)        // independent accumulators follow each other
 #pragma unroll
-      for (int t = 0; t < D / 32; ++t) S[t] = mfma(yf[t], part[i], S[t]);
+      for (int t = 0; t < 4; ++t) S[t] = L::mfma(yf[t], part[i], S[t]);
   }
 }
 
-// State tiles: wave w holds columns 32 w .. + 31; a lane column lane & 31, rows 32 t + 8 (r / 4) + 4 (lane / 32) + r % 4.
-template <int D>
-__device__ __forceinline__ void load_state(f32x16 (&S)[D / 32], const float* src, bool transposed, int wave, int lane) {
-  const int col = wave * 32 + (lane & 31), hh = lane >> 5;
+// State tiles: accumulator t holds rows W t .. of this wave's W columns.
+template <int D, int W = D / 4>
+__device__ __forceinline__ void load_state(typename Layout<W>::Acc (&S)[D / W], const float* src, bool transposed, int wave,
+                                           int lane) {
+  using L = Layout<W>;
+  const int col = wave * W + L::line(lane);
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < D / W; ++t)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int row = t * 32 + q * 8 + hh * 4;
+    for (int r = 0; r < W * W / 64; r += 4) {
+      const int row = t * W + L::row_of(lane, r);
       if (transposed) {
-        const float4 v = *(const float4*)(src + (long)col * D + row);
-        S[t][4 * q] = v.x; S[t][4 * q + 1] = v.y; S[t][4 * q + 2] = v.z; S[t][4 * q + 3] = v.w;
+        const f32x4 v = *(const f32x4*)(src + col * D + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[t][r + e] = v[e];
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) S[t][4 * q + e] = src[(long)(row + e) * D + col];
+        for (int e = 0; e < 4; ++e) S[t][r + e] = src[(row + e) * D + col];
       }
     }
 }
-template <int D>
-__device__ __forceinline__ void store_state(const f32x16 (&S)[D / 32], float* dst, int wave, int lane) {
-  const int col = wave * 32 + (lane & 31), hh = lane >> 5;
+template <int D, int W = D / 4>
+__device__ __forceinline__ void store_state(const typename Layout<W>::Acc (&S)[D / W], float* dst, int wave, int lane) {
+  using L = Layout<W>;
+  const int col = wave * W + L::line(lane);
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < D / W; ++t)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dst[(long)(t * 32 + (r >> 2) * 8 + hh * 4 + (r & 3)) * D + col] = S[t][r];
+    for (int r = 0; r < W * W / 64; ++r) dst[(t * W + L::row_of(lane, r)) * D + col] = S[t][r];
 }
 
 template <class T>
@@ -269,9 +396,9 @@ __device__ __forceinline__ const T* rows_at(const void* base, long ld, int group
 // segment's end, so the accumulators are only added to.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ __launch_bounds__(2 * D, 2) void linattn_sum_kernel(Params p) {
+__global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Params p) {
   using T = Tile<D>;
-  constexpr int DT = D / 32;
+  using L = LayoutOf<D>;
   extern __shared__ __align__(1024) uint8_t smem[];  // two stages of y and z, and the rows' weights of each
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Place w = place(p, p.n_sums);
@@ -280,11 +407,11 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_sum_kernel(Params p) {
   if (!ro.final_state && w.seg == (ro.reverse ? 0 : p.n_seg - 1)) return;
   const bf16_t* y = rows_at<bf16_t>(ro.y, ro.ldy, ro.gy, p, w, D);
   const bf16_t* z = rows_at<bf16_t>(ro.z, ro.ldz, ro.gz, p, w, D);
-  const uint32_t lds = lds_address(smem), unit = T::unit(), tr = tr_base(lane);
+  const uint32_t lds = lds_address(smem), unit = T::unit(), tr = L::tr(lane);
   const uint32_t offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
-  f32x16 S[DT];
+  typename L::Acc S[4];
 #pragma unroll
-  for (int t = 0; t < DT; ++t) S[t] = 0.f;
+  for (int t = 0; t < 4; ++t) S[t] = 0.f;
   const int n = (w.live + kChunk - 1) / kChunk;
   typename T::Regs ry, rz;
   auto fetch = [&](int c) {
@@ -305,9 +432,9 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_sum_kernel(Params p) {
     T::put(ztile + unit, rz);
     __syncthreads();       // (and nobody is still reading the stage that the next trip fills)
     if (c + 1 < n) fetch(c + 1);
-    bf16x8 zf[4];
+    bf16x8 zf[kChunk / L::K];
 #pragma unroll
-    for (int st = 0; st < 4; ++st) zf[st] = tr_frag(ztile + (wave >> 1) * 8192 + (tr ^ ((wave & 1) << 6)), 0, st);
+    for (int k = 0; k < kChunk / L::K; ++k) zf[k] = L::columns(ztile + tr, wave, k);
     update_state<D, 3>(S, ytile + tr, zf, up, lane);
   }
   store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
@@ -353,20 +480,24 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
 }
 
 // ---------------------------------------------------------------------------
-// the walk, bf16.  Per chunk: P^T = Y X^T in quadrants of 32 x 32 (weighted, in two bf16 parts, shared through
+// the walk, bf16.  Per chunk: P^T = Y X^T in accumulator tiles (weighted, in two bf16 parts, shared through
 // LDS); O^T = S^T X^T from the state's accumulators as they are, times the rows' decay, plus Z^T P^T; then the
 // state's update.
 // The state and the pairs meet the matrix cores as two bf16 each (16 bits): one would add, to
 // the rounding of the result, as much again.
+// The state is held over a factor m that takes the decays, so that most chunks leave the accumulators alone: m falls by
+// lambda^rows a chunk, the new terms are divided by it, and below 2^-20 it is multiplied in.
 // PARTS: of the state's terms, see update_state.
 // ---------------------------------------------------------------------------
 template <int D>
 constexpr int walk_lds() { return 3 * Tile<D>::BYTES + 2 * 8192 + (int)sizeof(Weights); }
 
 template <int D, int PARTS>
-__global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
+__global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Params p) {
   using T = Tile<D>;
-  constexpr int DT = D / 32, NW = D / 32;
+  using L = LayoutOf<D>;
+  typedef typename L::Acc Acc;
+  constexpr int W = D / 4, RT = kChunk / W, KC = kChunk / L::K;    // columns of a wave; row tiles and contraction steps of a chunk
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t xtile = lds_address(smem);          // later the chunk's result
   const uint32_t ytile = xtile + T::BYTES, ztile = ytile + T::BYTES;
@@ -374,7 +505,7 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
   Weights* const weights = (Weights*)(smem + 3 * T::BYTES + 2 * 8192);
   const uint32_t pair = lds_address(weights->pair), up = lds_address(weights->up), ofstate = lds_address(weights->state);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int hh = lane >> 5, li = lane & 31;
+  const int line = L::line(lane);
   const Place w = place(p, p.n_roles);
   const Role& ro = p.role[w.role];
   const bool rev = ro.reverse;
@@ -383,17 +514,16 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
   const bf16_t* z = rows_at<bf16_t>(ro.z, ro.ldz, ro.gz, p, w, D);
   const long bh = (long)w.b * p.heads + w.h;
 
-  f32x16 S[DT];
+  Acc S[4];
   const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
   if (from) {
     load_state<D>(S, from, p.n_seg == 1 ? ro.init_transposed : ro.parts_transposed, wave, lane);
   } else {
 #pragma unroll
-    for (int t = 0; t < DT; ++t) S[t] = 0.f;
+    for (int t = 0; t < 4; ++t) S[t] = 0.f;
   }
   const bool keep_last = p.n_seg == 1 && ro.final_state;
-  const uint32_t unit = T::unit(), tr = tr_base(lane);
-  const uint32_t row = slab_off(li, 0);              // unit c of row li (+ 32: 4096 further) is at row ^ c * 16
+  const uint32_t unit = T::unit(), tr = L::tr(lane), row = L::row(lane);
   const uint32_t offx = T::offset(ro.ldx), offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
 
   const int n = (w.live + kChunk - 1) / kChunk;
@@ -406,102 +536,93 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
   };
   if (n) fetch(0);
   pair_weights(weights, w.g2, ro.a_pair, rev);
-  // the quadrant of pairs that never counts stays zero
-  for (int k = threadIdx.x; k < 256; k += T::THREADS) {
-    const int part = k >> 7, r = k & 31, c = (k >> 5) & 3;
-    lds_put(ptile + part * 8192 + (rev ? 4096 : 0) + slab_off(r, (rev ? 0 : 4) + c), u32x4{0, 0, 0, 0});
-  }
+  // the tiles of pairs that never count stay zero
+  for (int k = threadIdx.x; k < 1024; k += T::THREADS) lds_put(ptile + k * 16, u32x4{0, 0, 0, 0});
+  __syncthreads();
+  float m = 1.f;
   for (int i = 0; i < n; ++i) {
     const int c = rev ? n - 1 - i : i;
     const int rows = min(kChunk, w.live - c * kChunk);
-    row_weights(weights, w.g2, ro.a_update, ro.a_state, rows, rev);
+    const float after = m * decay_pow(w.g2, rows);   // the state's factor behind this chunk
+    const bool settle = after < 0x1p-20f || after > 0x1p20f || (i + 1 == n && keep_last);
+    row_weights(weights, w.g2, settle ? ro.a_update : ro.a_update / after, ro.a_state * m, rows, rev);
     T::put(xtile + unit, rx);
     T::put(ytile + unit, ry);
     T::put(ztile + unit, rz);
     __syncthreads();
     if (i + 1 < n) fetch(i + 1);
 
-#pragma unroll
-    for (int q = 0; q < 4 / NW; ++q) {
-      const int jt = q * (NW / 2) + (wave >> 1), it = wave & 1;
-      if (rev ? jt < it : jt > it) continue;       // no pair of these rows counts
-      f32x16 s;
+    // the tiles on and below the diagonal (above, walking back)
+    for (int q = wave; q < RT * (RT + 1) / 2; q += 4) {
+      const int major = q < 1 ? 0 : q < 3 ? 1 : q < 6 ? 2 : 3, minor = q - major * (major + 1) / 2;
+      const int it = rev ? minor : major, jt = rev ? major : minor;
+      Acc s;
       s = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint32_t at = (row ^ ((ks & 3) * 32 + hh * 16)) + (ks >> 2) * 8192;
-        s = mfma(lds_get<bf16x8>(ytile + jt * 4096 + at), lds_get<bf16x8>(xtile + it * 4096 + at), s);
+      for (int k = 0; k < D / L::K; ++k) {
+        const uint32_t at = L::step(row, lane, k);
+        s = L::mfma(lds_get<bf16x8>(ytile + jt * W * 128 + at), lds_get<bf16x8>(xtile + it * W * 128 + at), s);
       }
-      const uint32_t far = pair + (64 + (it - jt) * 32 + li - hh * 4 - 27) * 4;
+      constexpr int LAST = W == 32 ? 27 : 3;       // of a lane's rows, from its first
+      const uint32_t far = pair + (64 + (it - jt) * W + line - L::row_of(lane, 0) - LAST) * 4;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= lds_get<float>(far + (27 - (r >> 2) * 8 - (r & 3)) * 4);
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        float v[8];
-        acc8(v, s, s2 * 8);
-        const uint32_t at = ptile + it * 4096 + (row ^ ((jt * 2 + s2) * 32 + hh * 16));
-        lds_put(at, split(v));
-        lds_put(at + 8192, nearest(v));
-      }
+      for (int r = 0; r < W * W / 64; ++r) s[r] *= lds_get<float>(far + (LAST - L::row_of(0, r)) * 4);
+      L::put_pairs(ptile + it * W * 128, row, lane, jt, s);
     }
 
-    f32x16 o[2];
-    o[0] = 0.f;
-    o[1] = 0.f;
+    Acc o[RT];
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int it = 0; it < RT; ++it) o[it] = 0.f;
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        float v[8];
-        acc8(v, S[t], s2 * 8);
-        const bf16x8 hi = split(v), lo = nearest(v);
-        // elements 32 t + 16 s2 + 4 hh .. + 3 of the rows, and the same 8 further on
-        const uint32_t a = xtile + (row ^ ((t & 1) * 64 + s2 * 32)) + (t >> 1) * 8192 + hh * 8;
-        const uint32_t b = xtile + (row ^ ((t & 1) * 64 + s2 * 32 + 16)) + (t >> 1) * 8192 + hh * 8;
+    for (int k = 0; k < D / L::K; ++k) {
+      float v[8];
+      L::take(v, S, k);
+      const bf16x8 hi = split(v), lo = nearest(v);
+      bf16x8 xf[RT];
 #pragma unroll
-        for (int it = 0; it < 2; ++it) {
-          const u32x2 first = lds_get<u32x2>(a + it * 4096), second = lds_get<u32x2>(b + it * 4096);
-          const bf16x8 xf = __builtin_bit_cast(bf16x8, u32x4{first.x, first.y, second.x, second.y});
-          o[it] = mfma(hi, xf, o[it]);
-          o[it] = mfma(lo, xf, o[it]);
-        }
-      }
+      for (int it = 0; it < RT; ++it) xf[it] = L::ordered(xtile + it * W * 128, row, lane, k);
 #pragma unroll
-    for (int it = 0; it < 2; ++it) o[it] *= lds_get<float>(ofstate + (it * 32 + li) * 4);
-    bf16x8 zf[4];
+      for (int it = 0; it < RT; ++it) o[it] = L::mfma(hi, xf[it], o[it]);
 #pragma unroll
-    for (int st = 0; st < 4; ++st) zf[st] = tr_frag(ztile + (wave >> 1) * 8192 + (tr ^ ((wave & 1) << 6)), 0, st);
+      for (int it = 0; it < RT; ++it) o[it] = L::mfma(lo, xf[it], o[it]);
+    }
+#pragma unroll
+    for (int it = 0; it < RT; ++it) o[it] *= lds_get<float>(ofstate + (it * W + line) * 4);
+    bf16x8 zf[KC];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) zf[k] = L::columns(ztile + tr, wave, k);
     __syncthreads();
 #pragma unroll
-    for (int st = 0; st < 4; ++st)
+    for (int part = 0; part < 2; ++part)
 #pragma unroll
-      for (int it = 0; it < 2; ++it) {
+      for (int k = 0; k < KC; ++k)
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
-          o[it] = mfma(zf[st], lds_get<bf16x8>(ptile + part * 8192 + it * 4096 + (row ^ (st * 32 + hh * 16))), o[it]);
-      }
+        for (int it = 0; it < RT; ++it)
+          o[it] = L::mfma(zf[k], lds_get<bf16x8>(ptile + part * 8192 + it * W * 128 + L::step(row, lane, k)), o[it]);
     if (ro.out_f32) {
-      float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D + wave * 32;
+      float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D + wave * W;
 #pragma unroll
-      for (int it = 0; it < 2; ++it)
-        if (it * 32 + li < rows)
+      for (int it = 0; it < RT; ++it)
+        if (it * W + line < rows)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *(float4*)(out + (long)(it * 32 + li) * ro.ldo + q * 8 + hh * 4) =
-                make_float4(o[it][4 * q], o[it][4 * q + 1], o[it][4 * q + 2], o[it][4 * q + 3]);
+          for (int q = 0; q < L::GROUPS; ++q)
+            *(f32x4*)(out + (long)(it * W + line) * ro.ldo + L::out_col(lane, q)) =
+                f32x4{o[it][4 * q], o[it][4 * q + 1], o[it][4 * q + 2], o[it][4 * q + 3]};
     } else {
       // x is no longer needed: its place takes the result, which leaves by whole rows
 #pragma unroll
-      for (int it = 0; it < 2; ++it)
+      for (int it = 0; it < RT; ++it)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          lds_put(xtile + (wave >> 1) * 8192 + it * 4096 + (row ^ ((wave & 1) * 64 + q * 16)) + hh * 8,
+        for (int q = 0; q < L::GROUPS; ++q)
+          lds_put(xtile + it * W * 128 + L::out(row, lane, wave, q),
                   u32x2{pack2(o[it][4 * q], o[it][4 * q + 1]), pack2(o[it][4 * q + 2], o[it][4 * q + 3])});
     }
     if (i + 1 < n || keep_last) {
-      const float keep = decay_pow(w.g2, rows);
+      if (settle) {
 #pragma unroll
-      for (int t = 0; t < DT; ++t) S[t] *= keep;
+        for (int t = 0; t < 4; ++t) S[t] *= after;
+      }
+      m = settle ? 1.f : after;
       update_state<D, PARTS>(S, ytile + tr, zf, up, lane);
     }
     __syncthreads();
@@ -511,7 +632,8 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
 #pragma unroll
       for (int k = 0; k < T::PER; ++k)
         // (the unit this thread overwrites with the next chunk's x)
-        if ((int)(threadIdx.x / T::UNITS) + 16 * k < rows) *(u32x4*)(out + 32 * k * ro.ldo + off) = lds_get<u32x4>(xtile + unit + k * 2048);
+        if ((int)(threadIdx.x / T::UNITS) + T::STEP * k < rows)
+          *(u32x4*)(out + 2 * T::STEP * k * ro.ldo + off) = lds_get<u32x4>(xtile + unit + k * T::STEP * 128);
     }
   }
   if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
@@ -524,100 +646,105 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_kernel(Params p) {
 }
 
 // ---------------------------------------------------------------------------
-// the same on f32 tensors: f32 MFMA (32x32x2), chunks of 32 rows, rows padded in LDS
+// the same on f32 tensors: f32 MFMA (16x16x4; a lane supplies one element, of row lane & 15 and contraction index
+// lane / 16, so that an accumulator's register r is an operand over the rows 4 g + r), chunks of 32 rows, rows padded in LDS
 // ---------------------------------------------------------------------------
 template <int D>
 struct TileF {
-  static constexpr int THREADS = 2 * D;
+  static constexpr int THREADS = 4 * D;
   static constexpr int LD = D + 4;                   // floats of a row: 16 bytes of padding turn the banks
-  static constexpr int BYTES = kChunkF32 * LD * 4;
   static constexpr int UNITS = D / 4;
   static constexpr int PER = kChunkF32 * UNITS / THREADS;
-  static __device__ __forceinline__ void load(float4 (&r)[PER], const float* src, long ld, int live) {
+  typedef f32x4 Regs[PER];
+  static __device__ __forceinline__ void load(Regs& r, const float* src, long ld, int live) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
-      r[i] = row < live ? *(const float4*)(src + row * ld + c * 4) : make_float4(0, 0, 0, 0);
+      r[i] = 0.f;
+      if (row < live) r[i] = *(const f32x4*)(src + row * ld + c * 4);
     }
   }
-  static __device__ __forceinline__ void put(float* tile, const float4 (&r)[PER]) {
+  static __device__ __forceinline__ void put(float* tile, const Regs& r) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
-      *(float4*)(tile + row * LD + c * 4) = r[i];
+      *(f32x4*)(tile + row * LD + c * 4) = r[i];
     }
   }
 };
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
 
-__device__ __forceinline__ float elem(const float4& v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; }
-
-// zf[r]: z of row 8 (r / 4) + 4 (lane / 32) + r % 4 at this lane's column
+// zf[4 jt + r]: z of row 16 jt + 4 g + r at this lane's column
 template <int D>
-__device__ __forceinline__ void update_state_f32(f32x16 (&S)[D / 32], const float* ytile, const float (&zf)[16], float g2,
-                                                 float a_update, int rows, bool reverse, int lane) {
-  const float keep = decay_pow(g2, rows);
+__device__ __forceinline__ void update_state_f32(f32x4 (&S)[D / 16], const float* ytile, const float (&zf)[8], const float* up,
+                                                 int lane) {
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) S[t] *= keep;
+  for (int r = 0; r < 8; ++r) {
+    const int j = (r >> 2) * 16 + (lane >> 4) * 4 + (r & 3);
+    const float z = zf[r] * up[j];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int j = (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
-    const float z = zf[r] * (a_update * decay_pow(g2, reverse ? j + 1 : max(rows - 1 - j, 0)));
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-      S[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(ytile[j * TileF<D>::LD + t * 32 + (lane & 31)], z, S[t], 0, 0, 0);
+    for (int t = 0; t < D / 16; ++t) S[t] = mfma_f32(ytile[j * TileF<D>::LD + t * 16 + (lane & 15)], z, S[t]);
   }
 }
 
 template <int D>
-__global__ __launch_bounds__(2 * D, 2) void linattn_sum_f32_kernel(Params p) {
+__global__ __launch_bounds__(4 * D, 4) void linattn_sum_f32_kernel(Params p) {
   using T = TileF<D>;
-  constexpr int DT = D / 32;
-  __shared__ __align__(16) float smem[2 * kChunkF32 * T::LD];
+  constexpr int DT = D / 16;
+  __shared__ __align__(16) float smem[2 * kChunkF32 * T::LD + kChunkF32];
   float* const ytile = smem;
   float* const ztile = smem + kChunkF32 * T::LD;
+  float* const up = smem + 2 * kChunkF32 * T::LD;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Place w = place(p, p.n_sums);
   const Role& ro = p.role[w.role];
   if (!ro.final_state && w.seg == (ro.reverse ? 0 : p.n_seg - 1)) return;
   const float* y = rows_at<float>(ro.y, ro.ldy, ro.gy, p, w, D);
   const float* z = rows_at<float>(ro.z, ro.ldz, ro.gz, p, w, D);
-  f32x16 S[DT];
+  f32x4 S[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) S[t] = 0.f;
   const int n = (w.live + kChunkF32 - 1) / kChunkF32;
-  float4 ry[T::PER], rz[T::PER];
-  auto fetch = [&](int i) {
-    const int c = ro.reverse ? n - 1 - i : i;
+  typename T::Regs ry, rz;
+  auto fetch = [&](int c) {
     T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, w.live - c * kChunkF32);
     T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, w.live - c * kChunkF32);
   };
   if (n) fetch(0);
-  for (int i = 0; i < n; ++i) {
-    const int c = ro.reverse ? n - 1 - i : i;
+  for (int c = 0; c < n; ++c) {
+    const int rows = min(kChunkF32, w.live - c * kChunkF32);
+    const int behind = ro.reverse ? c * kChunkF32 : w.live - c * kChunkF32 - rows;
+    if (threadIdx.x < kChunkF32) {
+      const int j = threadIdx.x;
+      up[j] = ro.a_update * decay_pow(w.g2, behind + (ro.reverse ? j + 1 : max(rows - 1 - j, 0)));
+    }
     T::put(ytile, ry);
     T::put(ztile, rz);
     __syncthreads();
-    if (i + 1 < n) fetch(i + 1);
-    float zf[16];
+    if (c + 1 < n) fetch(c + 1);
+    float zf[8];
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      zf[r] = ztile[((r >> 2) * 8 + (lane >> 5) * 4 + (r & 3)) * T::LD + wave * 32 + (lane & 31)];
-    update_state_f32<D>(S, ytile, zf, w.g2, ro.a_update, min(kChunkF32, w.live - c * kChunkF32), ro.reverse, lane);
+    for (int r = 0; r < 8; ++r) zf[r] = ztile[((r >> 2) * 16 + (lane >> 4) * 4 + (r & 3)) * T::LD + wave * 16 + (lane & 15)];
+    update_state_f32<D>(S, ytile, zf, up, lane);
     __syncthreads();
   }
-  store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
+  store_state<D, 16>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
 }
 
 template <int D>
-__global__ __launch_bounds__(2 * D, 2) void linattn_walk_f32_kernel(Params p) {
+__global__ __launch_bounds__(4 * D, 4) void linattn_walk_f32_kernel(Params p) {
   using T = TileF<D>;
-  constexpr int DT = D / 32;
-  __shared__ __align__(16) float smem[3 * kChunkF32 * T::LD];
+  constexpr int DT = D / 16, NW = D / 16, PLD = kChunkF32 + 4;
+  __shared__ __align__(16) float smem[3 * kChunkF32 * T::LD + kChunkF32 * PLD];
+  __shared__ Weights weights;
   float* const xtile = smem;
   float* const ytile = smem + kChunkF32 * T::LD;
   float* const ztile = smem + 2 * kChunkF32 * T::LD;
+  float* const ptile = smem + 3 * kChunkF32 * T::LD;    // rows i
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int hh = lane >> 5, li = lane & 31;
+  const int g = lane >> 4, li = lane & 15;
   const Place w = place(p, p.n_roles);
   const Role& ro = p.role[w.role];
   const bool rev = ro.reverse;
@@ -626,18 +753,17 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_f32_kernel(Params p) {
   const float* z = rows_at<float>(ro.z, ro.ldz, ro.gz, p, w, D);
   const long bh = (long)w.b * p.heads + w.h;
 
-  f32x16 S[DT];
+  f32x4 S[DT];
   const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
   if (from) {
-    load_state<D>(S, from, p.n_seg == 1 ? ro.init_transposed : ro.parts_transposed, wave, lane);
+    load_state<D, 16>(S, from, p.n_seg == 1 ? ro.init_transposed : ro.parts_transposed, wave, lane);
   } else {
 #pragma unroll
     for (int t = 0; t < DT; ++t) S[t] = 0.f;
   }
-  bool have_state = from != nullptr;
   const bool keep_last = p.n_seg == 1 && ro.final_state;
   const int n = (w.live + kChunkF32 - 1) / kChunkF32;
-  float4 rx[T::PER], ry[T::PER], rz[T::PER];
+  typename T::Regs rx, ry, rz;
   auto fetch = [&](int i) {
     const int c = rev ? n - 1 - i : i;
     T::load(rx, x + (long)c * kChunkF32 * ro.ldx, ro.ldx, w.live - c * kChunkF32);
@@ -645,52 +771,76 @@ __global__ __launch_bounds__(2 * D, 2) void linattn_walk_f32_kernel(Params p) {
     T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, w.live - c * kChunkF32);
   };
   if (n) fetch(0);
+  pair_weights(&weights, w.g2, ro.a_pair, rev);
   for (int i = 0; i < n; ++i) {
     const int c = rev ? n - 1 - i : i;
     const int rows = min(kChunkF32, w.live - c * kChunkF32);
+    row_weights(&weights, w.g2, ro.a_update, ro.a_state, rows, rev);
     T::put(xtile, rx);
     T::put(ytile, ry);
     T::put(ztile, rz);
     __syncthreads();
     if (i + 1 < n) fetch(i + 1);
-    // every wave for itself: the pairs, and what the state gives its columns
-    f32x16 s, o;
-    s = 0.f;
-    o = 0.f;
+    // the pairs: a wave a tile, the fourth is zero
+    if (wave < 4) {
+      const int it = wave & 1, jt = wave >> 1;
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+      if (rev ? jt >= it : jt <= it) {
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < DT; ++t) {
+          const f32x4 xv = *(const f32x4*)(xtile + (it * 16 + li) * T::LD + t * 16 + g * 4);
+          const f32x4 yv = *(const f32x4*)(ytile + (jt * 16 + li) * T::LD + t * 16 + g * 4);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int at = t * 32 + q * 8 + hh * 4;
-        const float4 xv = *(const float4*)(xtile + li * T::LD + at);
-        const float4 yv = *(const float4*)(ytile + li * T::LD + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s = __builtin_amdgcn_mfma_f32_32x32x2f32(elem(yv, e), elem(xv, e), s, 0, 0, 0);
-          o = __builtin_amdgcn_mfma_f32_32x32x2f32(S[t][4 * q + e], elem(xv, e), o, 0, 0, 0);
+          for (int e = 0; e < 4; ++e) s = mfma_f32(yv[e], xv[e], s);
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] *= weights.pair[64 + (it - jt) * 16 + li - g * 4 - r];
       }
-    if (have_state) o *= ro.a_state * decay_pow(w.g2, rev ? max(rows - 1 - li, 0) : li + 1);
-    float zf[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int j = (r >> 2) * 8 + hh * 4 + (r & 3);
-      const int far = rev ? j - li : li - j;
-      const float pair = far >= 0 ? s[r] * (ro.a_pair * decay_pow(w.g2, max(far, 0))) : 0.f;
-      zf[r] = ztile[j * T::LD + wave * 32 + li];
-      o = __builtin_amdgcn_mfma_f32_32x32x2f32(zf[r], pair, o, 0, 0, 0);
+      *(f32x4*)(ptile + (it * 16 + li) * PLD + jt * 16 + g * 4) = s;
     }
-    if (li < rows) {
-      float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunkF32 + li) * ro.ldo + (long)(w.h / ro.go) * D + wave * 32;
+    static_assert(NW >= 4, "a wave for every tile of pairs");
+    f32x4 o[2];
+    o[0] = 0.f;
+    o[1] = 0.f;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *(float4*)(out + q * 8 + hh * 4) = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+    for (int t = 0; t < DT; ++t) {
+      const f32x4 x0 = *(const f32x4*)(xtile + li * T::LD + t * 16 + g * 4);
+      const f32x4 x1 = *(const f32x4*)(xtile + (16 + li) * T::LD + t * 16 + g * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[0] = mfma_f32(S[t][e], x0[e], o[0]);
+        o[1] = mfma_f32(S[t][e], x1[e], o[1]);
+      }
     }
-    if (i + 1 < n || keep_last) update_state_f32<D>(S, ytile, zf, w.g2, ro.a_update, rows, rev, lane);
-    have_state = true;
+    o[0] *= weights.state[li];
+    o[1] *= weights.state[16 + li];
+    float zf[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) zf[r] = ztile[((r >> 2) * 16 + g * 4 + (r & 3)) * T::LD + wave * 16 + li];
+    __syncthreads();
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      const f32x4 p0 = *(const f32x4*)(ptile + li * PLD + jt * 16 + g * 4);
+      const f32x4 p1 = *(const f32x4*)(ptile + (16 + li) * PLD + jt * 16 + g * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[0] = mfma_f32(zf[4 * jt + e], p0[e], o[0]);
+        o[1] = mfma_f32(zf[4 * jt + e], p1[e], o[1]);
+      }
+    }
+    float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunkF32) * ro.ldo + (long)(w.h / ro.go) * D + wave * 16;
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+      if (it * 16 + li < rows) *(f32x4*)(out + (long)(it * 16 + li) * ro.ldo + g * 4) = o[it];
+    if (i + 1 < n || keep_last) {
+      const float keep = decay_pow(w.g2, rows);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) S[t] *= keep;
+      update_state_f32<D>(S, ytile, zf, weights.up, lane);
+    }
     __syncthreads();
   }
-  if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
+  if (keep_last) store_state<D, 16>(S, ro.final_state + bh * D * D, wave, lane);
   for (int k = threadIdx.x; k < (w.s1 - w.s0 - w.live) * T::UNITS; k += T::THREADS)
     *(float4*)((float*)ro.out + ((long)w.b * p.seq + w.s0 + w.live + k / T::UNITS) * ro.ldo + (long)(w.h / ro.go) * D +
                (k % T::UNITS) * 4) = make_float4(0, 0, 0, 0);
@@ -869,27 +1019,27 @@ int launch(hipStream_t st, const Params& p) {
     const unsigned carry = (unsigned)(sums * (D * D / 1024));
     const dim3 grid((unsigned)(sums * p.n_seg));
     if constexpr (F32) {
-      hipLaunchKernelGGL((linattn_sum_f32_kernel<D>), grid, dim3(2 * D), 0, st, p);
+      hipLaunchKernelGGL((linattn_sum_f32_kernel<D>), grid, dim3(4 * D), 0, st, p);
     } else {
       JPP_TRY(jpp_attn::set_smem(linattn_sum_kernel<D>, sum_lds<D>()));
-      hipLaunchKernelGGL((linattn_sum_kernel<D>), grid, dim3(2 * D), sum_lds<D>(), st, p);
+      hipLaunchKernelGGL((linattn_sum_kernel<D>), grid, dim3(256), sum_lds<D>(), st, p);
     }
     JPP_LAUNCH_CHECK();
     hipLaunchKernelGGL((linattn_carry_kernel<D>), dim3(carry), dim3(256), 0, st, p);
     JPP_LAUNCH_CHECK();
   }
   if constexpr (F32) {
-    hipLaunchKernelGGL((linattn_walk_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(2 * D), 0, st, p);
+    hipLaunchKernelGGL((linattn_walk_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(4 * D), 0, st, p);
   } else {
     bool last = false;           // a state that is a result comes out of the walk
     for (int i = 0; i < p.n_roles; ++i) last = last || (p.n_seg == 1 && p.role[i].final_state);
     const dim3 grid((unsigned)(walks * p.n_seg));
     if (last) {
       JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 3>, walk_lds<D>()));
-      hipLaunchKernelGGL((linattn_walk_kernel<D, 3>), grid, dim3(2 * D), walk_lds<D>(), st, p);
+      hipLaunchKernelGGL((linattn_walk_kernel<D, 3>), grid, dim3(256), walk_lds<D>(), st, p);
     } else {
       JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 2>, walk_lds<D>()));
-      hipLaunchKernelGGL((linattn_walk_kernel<D, 2>), grid, dim3(2 * D), walk_lds<D>(), st, p);
+      hipLaunchKernelGGL((linattn_walk_kernel<D, 2>), grid, dim3(256), walk_lds<D>(), st, p);
     }
   }
   JPP_LAUNCH_CHECK();
@@ -908,6 +1058,7 @@ Params params_of(const jpp_linattn_args* a, const Split& s) {
   p.batch = a->batch;
   p.seq = a->seq;
   p.heads = a->n_heads;
+  p.group = a->n_heads / a->n_kv_heads;
   p.n_seg = s.n;
   p.seg_rows = s.rows;
   return p;
