@@ -104,17 +104,17 @@ __device__ __forceinline__ Place place(const Params& p, int n_roles) {
 
 __device__ __forceinline__ float decay_pow(float g2, int n) { return exp2f(g2 * (float)n); }
 
-// Eight floats as the MFMA operand nearest to them (two elements per conversion), and, in place, what that leaves.
+// Two floats as the bf16 nearest to them, and, in place, what that leaves.
+__device__ __forceinline__ uint32_t split2(float& a, float& b) {
+  const uint32_t w = pack2(a, b);
+  a -= bf16lo_to_f32(w);
+  b -= bf16hi_to_f32(w);
+  return w;
+}
+// Eight floats as the MFMA operand nearest to them, and, in place, what that leaves.
 __device__ __forceinline__ bf16x8 split(float (&v)[8]) {
-  uint4 w;
-  uint32_t* const u = (uint32_t*)&w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    u[i] = pack2(v[2 * i], v[2 * i + 1]);
-    v[2 * i] -= bf16lo_to_f32(u[i]);
-    v[2 * i + 1] -= bf16hi_to_f32(u[i]);
-  }
-  return __builtin_bit_cast(bf16x8, w);
+  const uint32_t a = split2(v[0], v[1]), b = split2(v[2], v[3]), c = split2(v[4], v[5]), d = split2(v[6], v[7]);
+  return __builtin_bit_cast(bf16x8, make_uint4(a, b, c, d));
 }
 __device__ __forceinline__ bf16x8 nearest(const float (&v)[8]) {
   return __builtin_bit_cast(bf16x8, make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])));
@@ -168,6 +168,18 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < PER; ++i) lds_put(at + i * STEP * 128, r[i]);
   }
+  // with the middle halves of every two units changed over: their units then hold elements 0 - 3 and 8 - 11, and 4 - 7 and 12 - 15
+  static __device__ __forceinline__ uint32_t unit_crossed() {
+    const int c = threadIdx.x % UNITS;
+    return (c >> 3) * 8192 + slab_off(threadIdx.x / UNITS, c & 6) + (c & 1) * 8;
+  }
+  static __device__ __forceinline__ void put_crossed(uint32_t at, const Regs& r) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      lds_put(at + i * STEP * 128, u32x2{r[i].x, r[i].y});
+      lds_put((at ^ 16) + i * STEP * 128, u32x2{r[i].z, r[i].w});
+    }
+  }
 };
 
 // Two layouts of the same walk, both with four waves a workgroup: heads of 128 on 32 x 32 accumulators, a wave 32 columns
@@ -201,10 +213,15 @@ struct Layout<32> {
   static __device__ __forceinline__ uint32_t step(uint32_t row, int lane, int k) {       // rows' elements K k .. in memory order
     return (row ^ ((k & 3) * 32 + (lane >> 5) * 16)) + (k >> 2) * 8192;
   }
-  static __device__ __forceinline__ bf16x8 ordered(uint32_t tile, uint32_t row, int lane, int k) {   // and in the accumulators' order
-    const uint32_t at = tile + (k >> 2) * 8192 + (lane >> 5) * 8;
-    const u32x2 a = lds_get<u32x2>(at + (row ^ ((k & 3) * 32))), b = lds_get<u32x2>(at + (row ^ ((k & 3) * 32 + 16)));
-    return __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+  // and in the accumulators' order: x and y lie crossed in LDS, a unit is what a lane wants (as two halves of units, half of the
+  // banks lay idle)
+  static constexpr bool CROSSED = true;
+  static __device__ __forceinline__ bf16x8 ordered(uint32_t tile, uint32_t row, int lane, int k) {
+    return lds_get<bf16x8>(tile + step(row, lane, k));
+  }
+  static __device__ __forceinline__ uint32_t tr_crossed(int lane) {
+    const int g = lane >> 4, s = lane & 15;
+    return slab_off(((g >> 1) << 2) + (s >> 2), ((g & 1) << 1) + (s & 1)) + ((s >> 1) & 1) * 8;
   }
   // operand whose rows are a tile's columns 32 t .. and whose contraction runs over its rows 16 k .., in the accumulators' order;
   // `at` = the tile's address + tr(lane)
@@ -257,6 +274,8 @@ struct Layout<16> {
   static __device__ __forceinline__ uint32_t step(uint32_t row, int lane, int k) {
     return (row ^ ((k & 1) * 64 + (lane >> 4) * 16)) + (k >> 1) * 8192;
   }
+  static constexpr bool CROSSED = false;
+  static __device__ __forceinline__ uint32_t tr_crossed(int) { return 0; }
   static __device__ __forceinline__ bf16x8 ordered(uint32_t tile, uint32_t row, int lane, int k) {
     // elements 4 g .. + 3 are half of unit g / 2, 16 + 4 g .. of the next but one
     const uint32_t at = tile + (k >> 1) * 8192 + ((lane >> 4) & 1) * 8, unit = row ^ ((k & 1) * 64 + (lane >> 5) * 16);
@@ -299,10 +318,10 @@ __device__ __forceinline__ void Layout<32>::put_pairs(uint32_t at, uint32_t row,
 }
 __device__ __forceinline__ void Layout<16>::put_pairs(uint32_t at, uint32_t row, int lane, int jt, const Acc& s) {
   const uint32_t to = at + (row ^ ((jt >> 1) * 64 + (lane >> 4) * 16)) + (jt & 1) * 8;
-  const u32x2 hi = {pack2(s[0], s[1]), pack2(s[2], s[3])};
-  lds_put(to, hi);
-  lds_put(to + 8192, u32x2{pack2(s[0] - bf16lo_to_f32(hi.x), s[1] - bf16hi_to_f32(hi.x)),
-                           pack2(s[2] - bf16lo_to_f32(hi.y), s[3] - bf16hi_to_f32(hi.y))});
+  float v[4] = {s[0], s[1], s[2], s[3]};
+  const uint32_t a = split2(v[0], v[1]), b = split2(v[2], v[3]);
+  lds_put(to, u32x2{a, b});
+  lds_put(to + 8192, u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])});
 }
 // the layout of heads of D
 template <int D>
@@ -507,7 +526,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Par
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int line = L::line(lane);
   const Place w = place(p, p.n_roles);
-  const Role& ro = p.role[w.role];
+  const Role ro = p.role[w.role];
   const bool rev = ro.reverse;
   const bf16_t* x = rows_at<bf16_t>(ro.x, ro.ldx, ro.gx, p, w, D);
   const bf16_t* y = rows_at<bf16_t>(ro.y, ro.ldy, ro.gy, p, w, D);
@@ -524,7 +543,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Par
   }
   const bool keep_last = p.n_seg == 1 && ro.final_state;
   const uint32_t unit = T::unit(), tr = L::tr(lane), row = L::row(lane);
-  const uint32_t offx = T::offset(ro.ldx), offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
+  const uint32_t unit_xy = L::CROSSED ? T::unit_crossed() : unit, tr_y = L::CROSSED ? L::tr_crossed(lane) : tr;
+  const uint32_t offx = T::offset(ro.ldx), offy = T::offset(ro.ldy), offz = T::offset(ro.ldz), offo = T::offset(ro.ldo);
+  const long out_at = ((long)w.b * p.seq + w.s0) * ro.ldo + (long)(w.h / ro.go) * D;
 
   const int n = (w.live + kChunk - 1) / kChunk;
   typename T::Regs rx, ry, rz;
@@ -546,8 +567,13 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Par
     const float after = m * decay_pow(w.g2, rows);   // the state's factor behind this chunk
     const bool settle = after < 0x1p-20f || after > 0x1p20f || (i + 1 == n && keep_last);
     row_weights(weights, w.g2, settle ? ro.a_update : ro.a_update / after, ro.a_state * m, rows, rev);
-    T::put(xtile + unit, rx);
-    T::put(ytile + unit, ry);
+    if constexpr (L::CROSSED) {
+      T::put_crossed(xtile + unit_xy, rx);
+      T::put_crossed(ytile + unit_xy, ry);
+    } else {
+      T::put(xtile + unit, rx);
+      T::put(ytile + unit, ry);
+    }
     T::put(ztile + unit, rz);
     __syncthreads();
     if (i + 1 < n) fetch(i + 1);
@@ -600,7 +626,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Par
         for (int it = 0; it < RT; ++it)
           o[it] = L::mfma(zf[k], lds_get<bf16x8>(ptile + part * 8192 + it * W * 128 + L::step(row, lane, k)), o[it]);
     if (ro.out_f32) {
-      float* out = (float*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D + wave * W;
+      float* out = (float*)ro.out + out_at + (long)c * kChunk * ro.ldo + wave * W;
 #pragma unroll
       for (int it = 0; it < RT; ++it)
         if (it * W + line < rows)
@@ -623,17 +649,16 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Par
         for (int t = 0; t < 4; ++t) S[t] *= after;
       }
       m = settle ? 1.f : after;
-      update_state<D, PARTS>(S, ytile + tr, zf, up, lane);
+      update_state<D, PARTS>(S, ytile + tr_y, zf, up, lane);
     }
     __syncthreads();
     if (!ro.out_f32) {
-      uint8_t* out = (uint8_t*)((bf16_t*)ro.out + ((long)w.b * p.seq + w.s0 + c * kChunk) * ro.ldo + (long)(w.h / ro.go) * D);
-      const uint32_t off = T::offset(ro.ldo);
+      uint8_t* out = (uint8_t*)((bf16_t*)ro.out + out_at + (long)c * kChunk * ro.ldo);
 #pragma unroll
       for (int k = 0; k < T::PER; ++k)
-        // (the unit this thread overwrites with the next chunk's x)
+        // (a unit that this wave overwrites with the next chunk's x)
         if ((int)(threadIdx.x / T::UNITS) + T::STEP * k < rows)
-          *(u32x4*)(out + 2 * T::STEP * k * ro.ldo + off) = lds_get<u32x4>(xtile + unit + k * T::STEP * 128);
+          *(u32x4*)(out + 2 * T::STEP * k * ro.ldo + offo) = lds_get<u32x4>(xtile + unit + k * T::STEP * 128);
     }
   }
   if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
