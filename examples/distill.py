@@ -1,0 +1,249 @@
+"""A linear-attention student learns from a teacher's top logits, then generates token by token.
+
+    python examples/distill.py [--steps 30] [--layers 2] [--hidden 256] [--users 128]
+
+The student's layers mix tokens by linear attention with a decay for each head and are joined to the residual stream
+by gated norms: per layer
+
+    q, k, v = y Wqkv;  a = linattn(q, k, v) Wo;       h, y = join(h, a)
+    m = gelu(y W1) W2;                                h, y = join(h, m)
+
+and the loss is the distillation of its logits y Wout against the teacher's 16 largest (here a fixed random table of next
+tokens stands for the teacher).  Every tensor lives in device buffers and every operator is a call of
+``jaxpp_amd.runtime``, forward, backward and the Adam step.  Generation takes each user's prompt through the same
+forward, which leaves the layers' states, and then one token of every user at a time; its logits are compared with those of
+the whole text at once.  Needs an MI355X and the built library (`python -m jaxpp_amd.build`).
+"""
+from __future__ import annotations
+
+import argparse
+import ctypes
+import os
+import sys
+
+import numpy as np
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+from jaxpp_amd import runtime as rt          # noqa: E402
+
+EPS = 1e-6
+TOP = 16
+
+
+class Arena:
+    """Parameters as one flat tensor, with the gradients and the optimizer's state beside it."""
+
+    def __init__(self, shapes: dict, rng):
+        self.at, n = {}, 0
+        for name, shape in shapes.items():
+            self.at[name] = (n, shape)
+            n += int(np.prod(shape))
+        flat = np.empty(n, np.float32)
+        for name, (first, shape) in self.at.items():
+            size = int(np.prod(shape))
+            w = rng.standard_normal(size) / np.sqrt(shape[0]) if len(shape) == 2 else np.ones(size)
+            if "gate" in name:
+                w = 0.5 * w
+            flat[first:first + size] = w
+        self.n = n
+        self.master = rt.DeviceBuffer.from_numpy(flat)
+        self.param = rt.DeviceBuffer.from_f32_as_bf16(flat)
+        self.grad, self.m, self.v = (rt.DeviceBuffer(4 * n) for _ in range(3))
+        for b in (self.grad, self.m, self.v):
+            b.zero()
+
+    def w(self, name):
+        return self.param.ptr + 2 * self.at[name][0]
+
+    def g(self, name):
+        return self.grad.ptr + 4 * self.at[name][0]
+
+    def adam(self, step, lr):
+        rt.adam_step(self.n, self.grad.ptr, self.m.ptr, self.v.ptr, step, master=self.master.ptr, param=self.param.ptr,
+                     lr=lr, zero_grad=True)
+
+
+class Student:
+    """Buffers for `batch` sequences of `seq` rows; batch * seq a multiple of 128."""
+
+    def __init__(self, arena, layers, hidden, heads, ffn, vocab):
+        self.p, self.layers, self.hidden, self.heads, self.ffn, self.vocab = arena, layers, hidden, heads, ffn, vocab
+        self.dim = hidden // heads
+        self.decay = rt.DeviceBuffer.from_numpy(np.log1p(-2.0 ** -np.linspace(2, 7, heads)).astype(np.float32))
+
+    @staticmethod
+    def shapes(layers, hidden, ffn, vocab):
+        out = {}
+        for i in range(layers):
+            out.update({f"Wqkv{i}": (hidden, 3 * hidden), f"Wo{i}": (hidden, hidden), f"W1{i}": (hidden, ffn),
+                        f"b1{i}": (ffn,), f"W2{i}": (ffn, hidden)})
+            for j in ("a", "m"):
+                out.update({f"post_{j}{i}": (hidden,), f"gate_{j}{i}": (hidden,), f"pre_{j}{i}": (hidden,)})
+        out["Wout"] = (hidden, vocab)
+        return out
+
+    def buffers(self, batch, seq):
+        """What a forward of this size keeps for its backward."""
+        rows, bf16 = batch * seq, lambda cols: rt.DeviceBuffer(2 * batch * seq * cols)
+        keep = {"batch": batch, "seq": seq, "rows": rows, "h": [bf16(self.hidden)], "y": [bf16(self.hidden)], "rstd": [],
+                "logits": bf16(self.vocab), "layers": []}
+        for _ in range(self.layers):
+            keep["layers"].append({"qkv": bf16(3 * self.hidden), "o": bf16(self.hidden), "a": bf16(self.hidden),
+                                   "u": bf16(self.ffn), "s": bf16(self.ffn), "m": bf16(self.hidden)})
+            for _ in range(2):
+                keep["h"].append(bf16(self.hidden))
+                keep["y"].append(bf16(self.hidden))
+                keep["rstd"].append((rt.DeviceBuffer(4 * rows), rt.DeviceBuffer(4 * rows)))
+        need = max(rt.linattn_workspace(batch, seq, self.heads, self.heads, self.dim, b) for b in (False, True))
+        keep["workspace"] = rt.DeviceBuffer(max(need, 256))
+        keep["ones"] = rt.DeviceBuffer.from_f32_as_bf16(np.ones(self.hidden, np.float32))
+        return keep
+
+    def states(self, batch):
+        out = [rt.DeviceBuffer(4 * batch * self.heads * self.dim ** 2) for _ in range(self.layers)]
+        for b in out:
+            b.zero()
+        return out
+
+    def _qkv(self, buf, part):
+        return buf.ptr + 2 * part * self.hidden
+
+    def _join(self, keep, i, j, at, block):
+        p, (post, pre) = self.p, keep["rstd"][at]
+        rt.block_join_fwd(keep["h"][at].ptr, block.ptr, keep["h"][at + 1].ptr, keep["rows"], self.hidden,
+                          y=keep["y"][at + 1].ptr, gamma_post=p.w(f"post_{j}{i}"), gate=p.w(f"gate_{j}{i}"),
+                          gate_rows=keep["rows"], gamma_pre=p.w(f"pre_{j}{i}"), rstd_post=post.ptr, rstd_pre=pre.ptr, eps=EPS)
+
+    def forward(self, keep, embedded, states=None, single=False):
+        """`embedded`: [rows, hidden] float32.  `states`: taken and left, one per layer; `single`: one row per sequence."""
+        p, rows, hd, ff = self.p, keep["rows"], self.hidden, self.ffn
+        rt.copy_in([(np.ascontiguousarray(embedded, np.float32), keep["h"][0].ptr)], bf16=True)
+        norm = rt.NormArgs(keep["h"][0].ptr, keep["ones"].ptr, None, keep["y"][0].ptr, None, keep["rstd"][0][0].ptr,
+                           rows=rows, cols=hd, eps=EPS)
+        rt.check(rt.load().jpp_norm_fwd(None, ctypes.byref(norm)))
+        ld = (3 * hd,) * 3 + (hd,)
+        sizes = dict(batch=keep["batch"], n_heads=self.heads, n_kv_heads=self.heads, head_dim=self.dim, scale=self.dim ** -0.5)
+        for i, b in enumerate(keep["layers"]):
+            y = keep["y"][2 * i].ptr
+            rt.gemm(y, p.w(f"Wqkv{i}"), b["qkv"].ptr, rows, 3 * hd, hd, hd, 3 * hd, 3 * hd, 0, 1)
+            qkv = [self._qkv(b["qkv"], k) for k in range(3)]
+            if single:
+                rt.linattn_step(*qkv, b["o"].ptr, self.decay.ptr, states[i].ptr, states[i].ptr, *ld, **sizes)
+            else:
+                state = states[i].ptr if states else None
+                rt.linattn_fwd(*qkv, b["o"].ptr, self.decay.ptr, *ld, seq=keep["seq"], state_in=state, state_out=state,
+                               workspace=keep["workspace"].ptr, **sizes)
+            rt.gemm(b["o"].ptr, p.w(f"Wo{i}"), b["a"].ptr, rows, hd, hd, hd, hd, hd, 0, 1)
+            self._join(keep, i, "a", 2 * i, b["a"])
+            rt.gemm(keep["y"][2 * i + 1].ptr, p.w(f"W1{i}"), b["u"].ptr, rows, ff, hd, hd, ff, ff, 0, 1, rt.EPI_GELU,
+                    bias=p.w(f"b1{i}"), c2=b["s"].ptr, ldc2=ff)
+            rt.gemm(b["s"].ptr, p.w(f"W2{i}"), b["m"].ptr, rows, hd, ff, ff, hd, hd, 0, 1)
+            self._join(keep, i, "m", 2 * i + 1, b["m"])
+        rt.gemm(keep["y"][-1].ptr, p.w("Wout"), keep["logits"].ptr, rows, self.vocab, hd, hd, self.vocab, self.vocab, 0, 1)
+
+    def train_step(self, keep, grads, embedded, ids, teacher, weight, step, lr):
+        """One step; returns the loss."""
+        p, rows, hd, ff, vc = self.p, keep["rows"], self.hidden, self.ffn, self.vocab
+        self.forward(keep, embedded)
+        dev = [rt.DeviceBuffer.from_numpy(a) for a in (ids.astype(np.int32), teacher.astype(np.float32), weight)]
+        rt.distill_loss(keep["logits"].ptr, dev[0].ptr, dev[1].ptr, rows, vc, TOP, vc, grads["row_loss"].ptr,
+                        loss=grads["loss"].ptr, dlogits=keep["logits"].ptr, ldd=vc, weight=dev[2].ptr, temperature=2.0,
+                        scale=1.0 / weight.sum(), workspace=grads["distill"].ptr)
+        dlogits = keep["logits"].ptr              # the gradient takes the logits' place
+        rt.gemm(keep["y"][-1].ptr, dlogits, p.g("Wout"), hd, vc, rows, hd, vc, vc, 1, 1, rt.EPI_ACC_F32)
+        rt.gemm(dlogits, p.w("Wout"), grads["dy"].ptr, rows, hd, vc, vc, vc, hd, 0, 0)
+        dh = None
+
+        def join_bwd(i, j, at, block, dh):
+            post, pre = keep["rstd"][at]
+            rt.block_join_bwd(keep["h"][at + 1].ptr, block.ptr, dh, grads["dy"].ptr, grads["dh"].ptr, grads["db"].ptr, rows, hd,
+                              gamma_post=p.w(f"post_{j}{i}"), gate=p.w(f"gate_{j}{i}"), gate_rows=rows,
+                              gamma_pre=p.w(f"pre_{j}{i}"), rstd_post=post.ptr, rstd_pre=pre.ptr,
+                              dgamma_post=p.g(f"post_{j}{i}"), dgate=p.g(f"gate_{j}{i}"), dgamma_pre=p.g(f"pre_{j}{i}"),
+                              workspace=grads["join"].ptr)
+            return grads["dh"].ptr
+
+        for i in reversed(range(self.layers)):
+            b = keep["layers"][i]
+            dh = join_bwd(i, "m", 2 * i + 1, b["m"], dh)
+            db, y = grads["db"].ptr, keep["y"][2 * i + 1].ptr
+            rt.gemm(b["s"].ptr, db, p.g(f"W2{i}"), ff, hd, rows, ff, hd, hd, 1, 1, rt.EPI_ACC_F32)
+            rt.gemm(db, p.w(f"W2{i}"), grads["du"].ptr, rows, ff, hd, hd, hd, ff, 0, 0, rt.EPI_DGELU, aux=b["u"].ptr, ldaux=ff)
+            rt.gemm(y, grads["du"].ptr, p.g(f"W1{i}"), hd, ff, rows, hd, ff, ff, 1, 1, rt.EPI_ACC_F32)
+            rt.check(rt.load().jpp_colsum_accum(None, grads["du"].ptr, ff, rows, ff, p.g(f"b1{i}"), grads["colsum"].ptr))
+            rt.gemm(grads["du"].ptr, p.w(f"W1{i}"), grads["dy"].ptr, rows, hd, ff, ff, ff, hd, 0, 0)
+            dh = join_bwd(i, "a", 2 * i, b["a"], dh)
+            rt.gemm(b["o"].ptr, db, p.g(f"Wo{i}"), hd, hd, rows, hd, hd, hd, 1, 1, rt.EPI_ACC_F32)
+            rt.gemm(db, p.w(f"Wo{i}"), grads["do"].ptr, rows, hd, hd, hd, hd, hd, 0, 0)
+            qkv, dqkv = [self._qkv(b["qkv"], k) for k in range(3)], [self._qkv(grads["dqkv"], k) for k in range(3)]
+            rt.linattn_bwd(*qkv, grads["do"].ptr, *dqkv, self.decay.ptr, *(3 * hd,) * 3, hd, *(3 * hd,) * 3,
+                           batch=keep["batch"], seq=keep["seq"], n_heads=self.heads, n_kv_heads=self.heads, head_dim=self.dim,
+                           scale=self.dim ** -0.5, workspace=keep["workspace"].ptr)
+            rt.gemm(keep["y"][2 * i].ptr, grads["dqkv"].ptr, p.g(f"Wqkv{i}"), hd, 3 * hd, rows, hd, 3 * hd, 3 * hd, 1, 1,
+                    rt.EPI_ACC_F32)
+            rt.gemm(grads["dqkv"].ptr, p.w(f"Wqkv{i}"), grads["dy"].ptr, rows, hd, 3 * hd, 3 * hd, 3 * hd, hd, 0, 0)
+        p.adam(step, lr)
+        rt.sync()
+        return float(grads["loss"].download(np.float32, (1,))[0])
+
+    def gradient_buffers(self, batch, seq):
+        rows, bf16 = batch * seq, lambda cols: rt.DeviceBuffer(2 * batch * seq * cols)
+        ws = rt.load().jpp_workspace_bytes
+        return {"dy": bf16(self.hidden), "dh": bf16(self.hidden), "db": bf16(self.hidden), "do": bf16(self.hidden),
+                "du": bf16(self.ffn), "dqkv": bf16(3 * self.hidden), "row_loss": rt.DeviceBuffer(4 * rows),
+                "loss": rt.DeviceBuffer(4), "join": rt.DeviceBuffer(ws(7, self.hidden, 1, 0)),
+                "distill": rt.DeviceBuffer(max(ws(8, rows, 0, 0), 8)), "colsum": rt.DeviceBuffer(ws(1, self.ffn, 0, 0))}
+
+
+def main(argv=None):
+    ap = argparse.ArgumentParser()
+    ap.add_argument("--steps", type=int, default=30)
+    ap.add_argument("--layers", type=int, default=2)
+    ap.add_argument("--hidden", type=int, default=256)
+    ap.add_argument("--vocab", type=int, default=1024)
+    ap.add_argument("--batch", type=int, default=4)
+    ap.add_argument("--seq", type=int, default=160)
+    ap.add_argument("--users", type=int, default=128)
+    ap.add_argument("--prompt", type=int, default=9)
+    ap.add_argument("--tokens", type=int, default=4)
+    args = ap.parse_args(argv)
+    rt.require_gpu()
+    rng = np.random.default_rng(0)
+    hd, vc, ffn, heads = args.hidden, args.vocab, 2 * args.hidden, args.hidden // 64
+    embed = rng.standard_normal((vc, hd)).astype(np.float32)
+    table = 2 * rng.standard_normal((vc, vc)).astype(np.float32)          # the teacher: logits of the next token
+    best = np.argsort(-table, axis=1)[:, :TOP]
+    student = Student(Arena(Student.shapes(args.layers, hd, ffn, vc), rng), args.layers, hd, heads, ffn, vc)
+
+    keep, grads = student.buffers(args.batch, args.seq), student.gradient_buffers(args.batch, args.seq)
+    losses = []
+    for step in range(1, args.steps + 1):
+        text = rng.integers(0, vc, (args.batch, args.seq))
+        ids = best[text.reshape(-1)]
+        teacher = np.take_along_axis(table[text.reshape(-1)], ids, 1)
+        weight = np.ones((args.batch, args.seq), np.float32)
+        weight[:, :8] = 0                                                # a prompt carries no loss
+        losses.append(student.train_step(keep, grads, embed[text.reshape(-1)], ids, teacher, weight.reshape(-1), step, 3e-3))
+        if step == 1 or step % 10 == 0:
+            print(f"step {step:3d}: loss {losses[-1]:.4f}", flush=True)
+
+    # every user's prompt at once, then one token of each at a time - against the whole text at once
+    users, prompt, total = args.users, args.prompt, args.prompt + args.tokens
+    text = rng.integers(0, vc, (users, total))
+    whole = student.buffers(users, total)
+    student.forward(whole, embed[text.reshape(-1)])
+    want = whole["logits"].download_bf16((users, total, vc))
+    states, first, one = student.states(users), student.buffers(users, prompt), student.buffers(users, 1)
+    student.forward(first, embed[text[:, :prompt].reshape(-1)], states)
+    got = [first["logits"].download_bf16((users, prompt, vc))]
+    for t in range(prompt, total):
+        student.forward(one, embed[text[:, t]], states, single=True)
+        got.append(one["logits"].download_bf16((users, 1, vc)))
+    off = np.abs(np.concatenate(got, 1) - want).max() / np.sqrt(np.mean(want ** 2))
+    print(f"generation: largest difference {off:.2g} of the logits' rms over {args.tokens} tokens of {users} users")
+    return losses, off
+
+
+if __name__ == "__main__":
+    main()

@@ -56,6 +56,7 @@ struct Params {
   const float* decay;
   const int32_t* lens;
   int batch, seq, heads, group, n_seg, seg_rows;   // group: query heads per key head
+  int past;            // results go past the caches
 };
 
 struct Place {
@@ -128,6 +129,17 @@ template <class V> __device__ __forceinline__ void lds_put(uint32_t at, const V&
 }
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// a result past the caches, or through them
+template <class V> __device__ __forceinline__ void leave(V* to, const V& v, bool past) {
+  if (past) {
+    // (fenced in: two stores that differ in their hint alone are one to the compiler)
+    asm volatile("" ::: "memory");
+    __builtin_nontemporal_store(v, to);
+    asm volatile("" ::: "memory");
+  } else {
+    *to = v;
+  }
+}
 
 // ---------------------------------------------------------------------------
 // bf16 tiles: [64][D] in LDS as D / 64 swizzled slabs, staged through registers (rows behind
@@ -414,7 +426,7 @@ __device__ __forceinline__ const T* rows_at(const void* base, long ld, int group
 // sums of the segments: parts[seg] = what the segment adds to the state that leaves it.  Rows are weighted to the
 // segment's end, so the accumulators are only added to.
 // ---------------------------------------------------------------------------
-template <int D>
+template <int D, int PARTS>
 __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Params p) {
   using T = Tile<D>;
   using L = LayoutOf<D>;
@@ -432,29 +444,34 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Para
 #pragma unroll
   for (int t = 0; t < 4; ++t) S[t] = 0.f;
   const int n = (w.live + kChunk - 1) / kChunk;
-  typename T::Regs ry, rz;
-  auto fetch = [&](int c) {
-    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, offy, w.live - c * kChunk);
-    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, offz, w.live - c * kChunk);
+  typename T::Regs ry[2], rz[2];       // two chunks on their way
+  auto fetch = [&](int c, int at) {
+    T::load(ry[at], y + (long)c * kChunk * ro.ldy, ro.ldy, offy, w.live - c * kChunk);
+    T::load(rz[at], z + (long)c * kChunk * ro.ldz, ro.ldz, offz, w.live - c * kChunk);
   };
-  if (n) fetch(0);
-  for (int c = 0; c < n; ++c) {
+  auto chunk = [&](int c, int at) {
     const int rows = min(kChunk, w.live - c * kChunk);
-    const uint32_t ytile = lds + (c & 1) * (2 * T::BYTES + kChunk * 4), ztile = ytile + T::BYTES, up = ztile + T::BYTES;
+    const uint32_t ytile = lds + at * (2 * T::BYTES + kChunk * 4), ztile = ytile + T::BYTES, up = ztile + T::BYTES;
     // rows between this chunk and the end that the state leaves by
     const int behind = ro.reverse ? c * kChunk : w.live - c * kChunk - rows;
     if (threadIdx.x < kChunk) {
       const int j = threadIdx.x;
       lds_put(up + j * 4, ro.a_update * decay_pow(w.g2, behind + (ro.reverse ? j + 1 : max(rows - 1 - j, 0))));
     }
-    T::put(ytile + unit, ry);
-    T::put(ztile + unit, rz);
-    __syncthreads();       // (and nobody is still reading the stage that the next trip fills)
-    if (c + 1 < n) fetch(c + 1);
+    T::put(ytile + unit, ry[at]);
+    T::put(ztile + unit, rz[at]);
+    __syncthreads();       // (and nobody is still reading the stage that the next chunk fills)
+    if (c + 2 < n) fetch(c + 2, at);
     bf16x8 zf[kChunk / L::K];
 #pragma unroll
     for (int k = 0; k < kChunk / L::K; ++k) zf[k] = L::columns(ztile + tr, wave, k);
-    update_state<D, 3>(S, ytile + tr, zf, up, lane);
+    update_state<D, PARTS>(S, ytile + tr, zf, up, lane);
+  };
+  if (n > 0) fetch(0, 0);
+  if (n > 1) fetch(1, 1);
+  for (int c = 0; c < n; c += 2) {
+    chunk(c, 0);
+    if (c + 1 < n) chunk(c + 1, 1);
   }
   store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
 }
@@ -487,13 +504,24 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
     }
   }
   float* parts = ro.parts + (long)bh * p.n_seg * D * D + e;
-  for (int k = 0; k < p.n_seg; ++k) {
-    const int seg = ro.reverse ? p.n_seg - 1 - k : k;
-    float4* at = (float4*)(parts + (long)seg * D * D);
-    const float4 add = k + 1 < p.n_seg || ro.final_state ? *at : make_float4(0, 0, 0, 0);
-    *at = s;
-    const float keep = decay_pow(g2, min(max(len - seg * p.seg_rows, 0), p.seg_rows));
-    s = make_float4(s.x * keep + add.x, s.y * keep + add.y, s.z * keep + add.z, s.w * keep + add.w);
+  // the sums of eight segments are read ahead of the chain through them
+  constexpr int AHEAD = 8;
+  for (int k0 = 0; k0 < p.n_seg; k0 += AHEAD) {
+    float4 add[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int k = k0 + i, seg = ro.reverse ? p.n_seg - 1 - k : k;
+      add[i] = make_float4(0, 0, 0, 0);
+      if (k + 1 < p.n_seg || (k < p.n_seg && ro.final_state)) add[i] = *(const float4*)(parts + (long)seg * D * D);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int k = k0 + i, seg = ro.reverse ? p.n_seg - 1 - k : k;
+      if (k >= p.n_seg) break;
+      *(float4*)(parts + (long)seg * D * D) = s;
+      const float keep = decay_pow(g2, min(max(len - seg * p.seg_rows, 0), p.seg_rows));
+      s = make_float4(s.x * keep + add[i].x, s.y * keep + add[i].y, s.z * keep + add[i].z, s.w * keep + add[i].w);
+    }
   }
   if (ro.final_state) *(float4*)(ro.final_state + (long)bh * D * D + e) = s;
 }
@@ -658,7 +686,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Par
       for (int k = 0; k < T::PER; ++k)
         // (a unit that this wave overwrites with the next chunk's x)
         if ((int)(threadIdx.x / T::UNITS) + T::STEP * k < rows)
-          *(u32x4*)(out + 2 * T::STEP * k * ro.ldo + offo) = lds_get<u32x4>(xtile + unit + k * T::STEP * 128);
+          leave((u32x4*)(out + 2 * T::STEP * k * ro.ldo + offo), lds_get<u32x4>(xtile + unit + k * T::STEP * 128), p.past);
     }
   }
   if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
@@ -963,28 +991,43 @@ __global__ __launch_bounds__(256) void linattn_step_kernel(const E* q, const E* 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-constexpr int kSegUnit = 128;      // rows a segment is a multiple of
-constexpr int kMaxSegments = 64;
-
-// Workgroups that run at a time: by their LDS and registers two to a CU with heads of 128; with heads of 64, whose
-// workgroups have half the waves, three (bf16) or four (f32).
+// Workgroups that run at a time: by their LDS and registers two to a CU with heads of 128, three with heads of 64, four
+// there with f32 tensors.
 int slots_of(int head_dim, bool f32) { return 256 * (head_dim == 128 ? 2 : f32 ? 4 : 3); }
 
-// Rows of a segment for `walks` sequences x heads x roles.  A cut costs every segment the state's way in and out and a
-// pass over two of its three operands; it pays where whole rounds of workgroups get shorter by it.
-int segment_rows(int64_t walks, int64_t seq, int slots) {
+// Rows of a segment, by an estimate of the time in us: with R rounds of workgroups, each through `rows` rows, and X = 65536ths
+// of all walks' rows
+//   one segment   c0 + c1 R rows + c2 X
+//   n segments    c3 + c4 R rows + c5 X + c6 (n sums' states) / 512 + c7 n
+// (what a workgroup takes through its rows, what all share, the states' way out and in, the chain of the carry).
+// Least squares of the relative error over 200 problems of each kind, 1 .. 512 walks of 100 .. 16384 rows in 1 .. 64
+// segments; mean error 5 - 8 %.  Over those the choice costs 0.4 % (bf16) and 2 % (f32) over the best number of segments.  A segment has at
+// least 128 rows: below that its state is more to move than they are.
+// One head of 128, 4096 rows: 245 us in one segment, 36 in 32; 3 x 32 heads, 2048 rows: 128 in one, 84 in five.
+constexpr int kSegLeast = 128, kMaxSegments = 64;
+constexpr float kSegFit[2][2][8] = {   // [f32][head 128]
+    {{5.57f, 0.0372f, 2.46f, 10.8f, 0.0484f, 2.68f, 5.28f, 0.372f}, {5.14f, 0.0558f, 4.94f, 12.7f, 0.0774f, 4.52f, 18.7f, 0.35f}},
+    {{4.83f, 0.0701f, 7.07f, 10.5f, 0.1f, 9.25f, 4.48f, 0.367f}, {5.77f, 0.166f, 16.3f, 10.6f, 0.242f, 17.f, 17.7f, 0.344f}}};
+
+int segment_rows(const jpp_linattn_args* a, int roles, int sums) {
+  const bool f32 = a->dtype == JPP_DTYPE_F32;
+  const float* f = kSegFit[f32][a->head_dim == 128];
+  const int64_t seq = a->seq, heads = (int64_t)a->batch * a->n_heads, walks = heads * roles, slots = slots_of(a->head_dim, f32);
+  const int unit = f32 ? kChunkF32 : kChunk;
+  const float x = (float)(walks * seq) / 65536.f;
   int64_t best = std::max<int64_t>(seq, 1);
-  double least = 0;
-  for (int n = 1; n <= kMaxSegments; ++n) {
-    const int64_t rows = n == 1 ? std::max<int64_t>(seq, 1) : (seq + n * kSegUnit - 1) / (n * kSegUnit) * kSegUnit;
+  float least = f[0] + f[1] * (float)((walks + slots - 1) / slots * seq) + f[2] * x;
+  for (int64_t n = 2; n <= kMaxSegments; ++n) {
+    const int64_t rows = (seq + n * unit - 1) / (n * unit) * unit;
+    if (rows < kSegLeast) break;
+    if (rows >= seq) continue;
     const int64_t segs = (seq + rows - 1) / rows;
-    const double rounds = (double)((walks * segs + slots - 1) / slots);
-    const double time = rounds * (n == 1 ? rows + 64. : 1.6 * rows + 256.) + (n == 1 ? 0. : 256.);
-    if (n == 1 || time < least) {
+    const float time = f[3] + f[4] * (float)((walks * segs + slots - 1) / slots * rows) + f[5] * x +
+                       f[6] * (float)(heads * sums * segs) / 512.f + f[7] * (float)segs;
+    if (time < least) {
       least = time;
       best = rows;
     }
-    if (rows <= kSegUnit) break;
   }
   return (int)best;
 }
@@ -996,7 +1039,7 @@ struct Split {
 };
 Split split_of(const jpp_linattn_args* a, int roles) {
   Split s;
-  s.rows = segment_rows((int64_t)a->batch * a->n_heads * roles, a->seq, slots_of(a->head_dim, a->dtype == JPP_DTYPE_F32));
+  s.rows = segment_rows(a, roles, roles > 1 ? 2 : 1);
   s.n = std::max(1, (a->seq + s.rows - 1) / s.rows);     // (no rows: a walk that hands the state on)
   const size_t states = (size_t)a->batch * a->n_heads * a->head_dim * a->head_dim * 4;
   s.parts = s.n > 1 ? states * s.n : 0;
@@ -1046,8 +1089,15 @@ int launch(hipStream_t st, const Params& p) {
     if constexpr (F32) {
       hipLaunchKernelGGL((linattn_sum_f32_kernel<D>), grid, dim3(4 * D), 0, st, p);
     } else {
-      JPP_TRY(jpp_attn::set_smem(linattn_sum_kernel<D>, sum_lds<D>()));
-      hipLaunchKernelGGL((linattn_sum_kernel<D>), grid, dim3(256), sum_lds<D>(), st, p);
+      bool last = false;         // a state that is a result comes out of the sums
+      for (int i = 0; i < p.n_sums; ++i) last = last || p.role[i].final_state;
+      if (last) {
+        JPP_TRY(jpp_attn::set_smem(linattn_sum_kernel<D, 3>, sum_lds<D>()));
+        hipLaunchKernelGGL((linattn_sum_kernel<D, 3>), grid, dim3(256), sum_lds<D>(), st, p);
+      } else {
+        JPP_TRY(jpp_attn::set_smem(linattn_sum_kernel<D, 2>, sum_lds<D>()));
+        hipLaunchKernelGGL((linattn_sum_kernel<D, 2>), grid, dim3(256), sum_lds<D>(), st, p);
+      }
     }
     JPP_LAUNCH_CHECK();
     hipLaunchKernelGGL((linattn_carry_kernel<D>), dim3(carry), dim3(256), 0, st, p);
@@ -1084,6 +1134,9 @@ Params params_of(const jpp_linattn_args* a, const Split& s) {
   p.seq = a->seq;
   p.heads = a->n_heads;
   p.group = a->n_heads / a->n_kv_heads;
+  // Results of more than the caches keep for whoever comes next go past them, and leave them to what is read twice (16 x 512 rows
+  // of 32 heads of 128, 67 MB: 83 -> 72 us).
+  p.past = (int64_t)a->batch * a->seq * a->n_heads * a->head_dim >= (int64_t)16 << 20;
   p.n_seg = s.n;
   p.seg_rows = s.rows;
   return p;
