@@ -535,12 +535,14 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
 // The state is held over a factor m that takes the decays, so that most chunks leave the accumulators alone: m falls by
 // lambda^rows a chunk, the new terms are divided by it, and below 2^-20 it is multiplied in.
 // PARTS: of the state's terms, see update_state.
+// Three workgroups of heads of 64 fit a CU's LDS; registers for a fourth would be spilled ones (gradients of 2 x 4096 x 32
+// heads of 64 on 8: 128 us, 112 like this).
 // ---------------------------------------------------------------------------
 template <int D>
 constexpr int walk_lds() { return 3 * Tile<D>::BYTES + 2 * 8192 + (int)sizeof(Weights); }
 
 template <int D, int PARTS>
-__global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Params p) {
+__global__ __launch_bounds__(256, D == 128 ? 2 : 3) void linattn_walk_kernel(Params p) {
   using T = Tile<D>;
   using L = LayoutOf<D>;
   typedef typename L::Acc Acc;
@@ -646,21 +648,30 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_walk_kernel(Par
 #pragma unroll
     for (int k = 0; k < KC; ++k) zf[k] = L::columns(ztile + tr, wave, k);
     __syncthreads();
+    // (step k counts for rows it in both directions, in one, or in none)
+    auto pairs = [&](bool ahead, bool back) {
 #pragma unroll
-    for (int part = 0; part < 2; ++part)
+      for (int part = 0; part < 2; ++part)
 #pragma unroll
-      for (int k = 0; k < KC; ++k)
+        for (int k = 0; k < KC; ++k)
 #pragma unroll
-        for (int it = 0; it < RT; ++it)
-          o[it] = L::mfma(zf[k], lds_get<bf16x8>(ptile + part * 8192 + it * W * 128 + L::step(row, lane, k)), o[it]);
+          for (int it = 0; it < RT; ++it)
+            if ((L::K * k < W * (it + 1)) == ahead && (L::K * (k + 1) > W * it) == back)
+              o[it] = L::mfma(zf[k], lds_get<bf16x8>(ptile + part * 8192 + it * W * 128 + L::step(row, lane, k)), o[it]);
+    };
+    pairs(true, true);
+    if (rev) pairs(false, true);
+    else pairs(true, false);
     if (ro.out_f32) {
       float* out = (float*)ro.out + out_at + (long)c * kChunk * ro.ldo + wave * W;
+      int at = line;             // (addresses made here, not kept)
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int it = 0; it < RT; ++it)
-        if (it * W + line < rows)
+        if (it * W + at < rows)
 #pragma unroll
           for (int q = 0; q < L::GROUPS; ++q)
-            *(f32x4*)(out + (long)(it * W + line) * ro.ldo + L::out_col(lane, q)) =
+            *(f32x4*)(out + (long)(it * W + at) * ro.ldo + L::out_col(lane, q)) =
                 f32x4{o[it][4 * q], o[it][4 * q + 1], o[it][4 * q + 2], o[it][4 * q + 3]};
     } else {
       // x is no longer needed: its place takes the result, which leaves by whole rows
