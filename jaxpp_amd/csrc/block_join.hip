@@ -11,7 +11,7 @@
 //
 // HBM-bound: forward reads two tensors and writes two, backward reads four and writes two.  A row lives in
 // the registers of one wave or of one workgroup between its reductions.  bf16: 16384 x 4096 forward 98 us, 5.5 TB/s;
-// 8192 x 8192 backward 187 us and 11 for the lines' sums, 4.3 TB/s.
+// 8192 x 8192 backward 162 us, the lines' sums included, 5.0 TB/s.
 #include <math.h>
 
 #include <algorithm>
@@ -21,7 +21,7 @@
 namespace {
 
 constexpr int kMaxCols = 8192;
-constexpr int kJoinParts = 512;     // workgroups of a backward, each with a line of partial sums
+constexpr int kJoinParts = 512;     // workgroups of a backward at most (or one a gate row), each with a line of partial sums
 
 // 16 bytes of a row as floats and back
 template <class E> struct Unit;
@@ -61,6 +61,7 @@ struct JoinParams {
   float *rstd_post, *rstd_pre, *sum_e, *sum_f;
   long rows, gate_rows;
   int cols, splits;
+  int past;           // dx and db go past the caches
   float alpha, eps;
 };
 
@@ -137,6 +138,18 @@ __global__ __launch_bounds__(256) void block_join_fwd_kernel(JoinParams p) {
   }
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void leave(uint4* to, const uint4& v, int past) {
+  if (past) {
+    // (fenced in: two stores that differ in their hint alone are one to the compiler)
+    asm volatile("" ::: "memory");
+    __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, (u32x4*)to);
+    asm volatile("" ::: "memory");
+  } else {
+    *to = v;
+  }
+}
+
 // Workgroup `part` of a gate row's `splits`: its share of that row's rows, and one line of the sums E and F over them.
 // The next row's operands are on their way while a row is worked on.
 constexpr int bwd_threads(int tpr) { return tpr > 256 ? tpr : 256; }
@@ -178,7 +191,29 @@ __global__ __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 4 : 2) void block_joi
   // (units beyond the row stay zero and add nothing)
 #pragma unroll
   for (int i = 0; i < NCH; ++i) nb[i] = nh[i] = ny[i] = nd[i] = make_uint4(0, 0, 0, 0);
+  // The vectors over columns stay in registers: loads of theirs in each row would be waited for behind the next row's (8192 x 8192
+  // bf16: 200 us, 177 like this).
+  uint4 wpre[NCH], wpost[NCH], wgate[NCH];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int c = t + TPR * i;
+    wpre[i] = wpost[i] = wgate[i] = make_uint4(0, 0, 0, 0);
+    if (c < units) {
+      if (PRE) wpre[i] = ((const uint4*)p.gamma_pre)[c];
+      if (POST) wpost[i] = ((const uint4*)p.gamma_post)[c];
+      if (gr) wgate[i] = gr[c];
+    }
+  }
   if (first + lane < last) fetch(first + lane);
+  float wout[NCH][N];              // gate gamma_post
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    float w[N], g[N];
+    Unit<E>::get(wpost[i], w);
+    Unit<E>::get(wgate[i], g);
+#pragma unroll
+    for (int e = 0; e < N; ++e) wout[i][e] = (POST ? w[e] : 1.f) * (gr ? g[e] : 1.f);
+  }
   int turn = 0;
   for (long row = first + lane; row < last; row += LANES, turn ^= 32) {
     const long at = row * p.cols;
@@ -196,14 +231,10 @@ __global__ __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 4 : 2) void block_joi
         Unit<E>::get(nd[i], total[i]);
       }
       if (row + LANES < last) fetch(row + LANES);
-      uint4 vw[NCH];
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
-        const int c = t + TPR * i;
-        vw[i] = make_uint4(0, 0, 0, 0);
-        if (c < units) vw[i] = ((const uint4*)p.gamma_pre)[c];
         float w[N], h[N], y[N];
-        Unit<E>::get(vw[i], w);
+        Unit<E>::get(wpre[i], w);
         Unit<E>::get(vh[i], h);
         Unit<E>::get(vy[i], y);
 #pragma unroll
@@ -217,7 +248,7 @@ __global__ __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 4 : 2) void block_joi
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         float w[N], h[N], y[N];
-        Unit<E>::get(vw[i], w);
+        Unit<E>::get(wpre[i], w);
         Unit<E>::get(vh[i], h);
         Unit<E>::get(vy[i], y);
 #pragma unroll
@@ -235,30 +266,17 @@ __global__ __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 4 : 2) void block_joi
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int c = t + TPR * i;
-      float b[N], dx[N], w[N];
+      float b[N], dx[N];
       Unit<E>::get(vb[i], b);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         dx[e] = p.alpha * total[i][e];
         if (POST) b[e] *= rb;
         se[i][e] += total[i][e] * b[e];
+        total[i][e] *= wout[i][e];
+        if (POST) s += total[i][e] * b[e];
       }
-      if (c < units) {
-        ((uint4*)((E*)p.dx + at))[c] = Unit<E>::put(dx);
-        if (gr) {
-          Unit<E>::get(gr[c], w);
-#pragma unroll
-          for (int e = 0; e < N; ++e) total[i][e] *= w[e];
-        }
-        if (POST) {
-          Unit<E>::get(((const uint4*)p.gamma_post)[c], w);
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            total[i][e] *= w[e];
-            s += total[i][e] * b[e];
-          }
-        }
-      }
+      if (c < units) leave((uint4*)((E*)p.dx + at) + c, Unit<E>::put(dx), p.past);
     }
     if (POST) s = row_sum<TPR>(s, lds + turn + 16) / p.cols;
 #pragma unroll
@@ -271,7 +289,7 @@ __global__ __launch_bounds__(bwd_threads(TPR), TPR > 256 ? 4 : 2) void block_joi
 #pragma unroll
           for (int e = 0; e < N; ++e) total[i][e] = rb * (total[i][e] - b[e] * rb * s);
         }
-        ((uint4*)((E*)p.db + at))[c] = Unit<E>::put(total[i]);
+        leave((uint4*)((E*)p.db + at) + c, Unit<E>::put(total[i]), p.past);
       }
     }
   }
@@ -428,8 +446,8 @@ int forward(hipStream_t st, const JoinParams& p) {
 }
 
 // Backward: one unit a thread, so that a row, the next row and the sums fit the registers of twice the waves (8192 rows of
-// 8192 bf16: 187 us with 1024 threads of one unit, 204 with 512 of two and half the waves on a CU, 540 and more with
-// 256 of four, which spill).
+// 8192 bf16, before the vectors stayed in registers: 187 us with 1024 threads of one unit, 204 with 512 of two and half the waves on a
+// CU, 540 and more with 256 of four, which spill).
 template <class E, bool PRE, bool POST>
 int backward_rows(hipStream_t st, const JoinParams& p, long lines) {
   const int units = p.cols / Unit<E>::N;
@@ -451,7 +469,13 @@ template <class E>
 int backward(hipStream_t st, JoinParams p, const jpp_join_args* a) {
   const long groups = p.rows / p.gate_rows;
   const bool sums = a->dgamma_post || a->dgate || a->dgamma_pre;
-  p.splits = (int)std::min<long>(groups >= kJoinParts ? 1 : (kJoinParts + groups - 1) / groups, p.gate_rows);
+  // Rows of 512 threads and more: a workgroup a CU, so that fewer lines are left to sum (8192 x 8192 bf16 172 us with two, 162 with one;
+  // 16384 x 4096 166 and 163); of fewer threads two (32768 x 768: 57 us, 61 with one; 16384 x 2048: 88 and 92).
+  const long parts = p.cols / Unit<E>::N > 256 ? kJoinParts / 2 : kJoinParts;
+  p.splits = (int)std::min<long>(groups >= parts ? 1 : (parts + groups - 1) / groups, p.gate_rows);
+  // Gradients of more than the caches keep for whoever comes next go past them (8192 x 4096 bf16, 67 MB each: 90 us, 71 like
+  // this; 16384 x 4096 f32: 320 and 330).
+  p.past = p.rows * p.cols >= (long)16 << 20;
   p.sum_e = sums ? (float*)a->workspace : nullptr;
   p.sum_f = sums ? p.sum_e + groups * p.splits * p.cols : nullptr;
   const long lines = groups * p.splits;
