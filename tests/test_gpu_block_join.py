@@ -226,3 +226,9 @@ def test_repeats_are_bit_identical_on_another_stream_and_in_a_graph():
     for got in runs:
         for n in want:
             np.testing.assert_array_equal(got[n], want[n], err_msg=n)
+
+
+@pytest.mark.parametrize("rows,cols,f32", [(2056, 8192, False), (16392, 1024, False), (4112, 4096, True)])
+def test_gradients_of_more_than_the_caches(rows, cols, f32):
+    """Gradients of 16 M elements and more are stored past the caches; a workgroup has several rows."""
+    Problem(rows, cols, f32, gate_rows=rows // 2, seed=6).check_backward()

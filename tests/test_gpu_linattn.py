@@ -311,3 +311,18 @@ def test_another_stream_repeats_and_graphs():
     for _ in range(3):
         graph.launch()
         check()
+
+
+@pytest.mark.parametrize("heads,dim,seq", [(64, 128, 2049), (128, 64, 2049)])
+def test_results_of_more_than_the_caches(heads, dim, seq):
+    """Results of 16 M elements and more are stored past the caches; a few heads are looked at, which is all a head can tell."""
+    p = Problem(1, seq, heads, heads, dim, states=False, seed=5)
+    pick = [0, heads // 3, heads - 1]
+    q, k, v, d_o = (a[:, :, pick] for a in (p.q, p.k, p.v, p.d_o))
+    args = (p.decay[pick], p.sizes["scale"])
+    sizes = [np.abs(a) for a in (q, k, v, d_o)]
+    o, _ = p.forward()
+    _close(o[:, :, pick], O.linattn(q, k, v, *args, None, None)[0], O.linattn(*sizes[:3], *args, None, None)[0], False, "o")
+    want, size = O.linattn_bwd(q, k, v, d_o, *args, None, None, None), O.linattn_bwd(*sizes, *args, None, None, None)
+    for name, got, w, m in zip(("dq", "dk", "dv"), p.backward(), want, size):
+        _close(got[:, :, pick], w, m, False, name)
