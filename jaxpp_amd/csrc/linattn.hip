@@ -145,6 +145,8 @@ template <class V> __device__ __forceinline__ void leave(V* to, const V& v, bool
 // bf16 tiles: [64][D] in LDS as D / 64 swizzled slabs, staged through registers (rows behind
 // the sequence's end are not read and count as zero)
 // ---------------------------------------------------------------------------
+constexpr int kBuffer = 0x00027000;      // a buffer of 32-bit elements, no swizzle (word 3 of its description)
+
 template <int D>
 struct Tile {
   static constexpr int THREADS = 256;
@@ -162,18 +164,15 @@ struct Tile {
     const int c = threadIdx.x % UNITS;
     return (c >> 3) * 8192 + slab_off(threadIdx.x / UNITS, c & 7);
   }
+  // Rows from `live` on are out of the buffer's range, read nothing and count as zero.  (A branch per row had every load in
+  // flight waited for, since their number was not known: sums of 2 x 4096 rows of 32 heads on 8 60 us, 52 like this.)
   static __device__ __forceinline__ void load(Regs& r, const bf16_t* src, long ld, uint32_t off, int live) {
-    const uint8_t* base = (const uint8_t*)src;
-    if (live >= kChunk) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) r[i] = *(const u32x4*)(base + 2 * STEP * i * ld + off);
-    } else {
-      const int row = threadIdx.x / UNITS;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        r[i] = u32x4{0, 0, 0, 0};
-        if (row + STEP * i < live) r[i] = *(const u32x4*)(base + 2 * STEP * i * ld + off);
-      }
+    for (int i = 0; i < PER; ++i) {
+      const int rows = min(max(live - STEP * i, 0), STEP);
+      const int bytes = __builtin_amdgcn_readfirstlane(rows ? (int)((uint32_t)((rows - 1) * ld + D) * 2) : 0);
+      r[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+          __builtin_amdgcn_make_buffer_rsrc((void*)(src + STEP * i * ld), 0, bytes, kBuffer), off, 0, 0));
     }
   }
   static __device__ __forceinline__ void put(uint32_t at, const Regs& r) {
@@ -392,20 +391,21 @@ __device__ __forceinline__ void load_state(typename Layout<W>::Acc (&S)[D / W], 
                                            int lane) {
   using L = Layout<W>;
   const int col = wave * W + L::line(lane);
+  if (transposed) {          // (two loops: a choice for each load has every one waited for)
 #pragma unroll
-  for (int t = 0; t < D / W; ++t)
+    for (int t = 0; t < D / W; ++t)
 #pragma unroll
-    for (int r = 0; r < W * W / 64; r += 4) {
-      const int row = t * W + L::row_of(lane, r);
-      if (transposed) {
-        const f32x4 v = *(const f32x4*)(src + col * D + row);
+      for (int r = 0; r < W * W / 64; r += 4) {
+        const f32x4 v = *(const f32x4*)(src + col * D + t * W + L::row_of(lane, r));
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[t][r + e] = v[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[t][r + e] = src[(row + e) * D + col];
       }
-    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < D / W; ++t)
+#pragma unroll
+      for (int r = 0; r < W * W / 64; ++r) S[t][r] = src[(t * W + L::row_of(lane, r)) * D + col];
+  }
 }
 template <int D, int W = D / 4>
 __device__ __forceinline__ void store_state(const typename Layout<W>::Acc (&S)[D / W], float* dst, int wave, int lane) {
@@ -425,7 +425,7 @@ __device__ __forceinline__ const T* rows_at(const void* base, long ld, int group
 // ---------------------------------------------------------------------------
 // sums of the segments: parts[seg] = what the segment adds to the state that leaves it.  Rows are weighted to the
 // segment's end, so the accumulators are only added to.  Rows of two chunks ahead are on their way (16384 rows of 32 heads of 128:
-// 57 us, 4.7 TB/s; 69 with terms in three parts, the matrix cores' time).
+// 56 us, 4.8 TB/s; 69 with terms in three parts, the matrix cores' time).
 // ---------------------------------------------------------------------------
 template <int D, int PARTS>
 __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Params p) {
@@ -462,18 +462,21 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Para
     T::put(ytile + unit, ry[at]);
     T::put(ztile + unit, rz[at]);
     __syncthreads();       // (and nobody is still reading the stage that the next chunk fills)
-    if (c + 2 < n) fetch(c + 2, at);
+    fetch(c + 2, at);      // (behind the last one: nothing)
     bf16x8 zf[kChunk / L::K];
 #pragma unroll
     for (int k = 0; k < kChunk / L::K; ++k) zf[k] = L::columns(ztile + tr, wave, k);
     update_state<D, PARTS>(S, ytile + tr, zf, up, lane);
   };
-  if (n > 0) fetch(0, 0);
-  if (n > 1) fetch(1, 1);
-  for (int c = 0; c < n; c += 2) {
+  fetch(0, 0);
+  asm volatile("" ::: "memory");       // (in this order, as in the loop: what is waited for is counted)
+  fetch(1, 1);
+  int c = 0;
+  for (; c + 1 < n; c += 2) {
     chunk(c, 0);
-    if (c + 1 < n) chunk(c + 1, 1);
+    chunk(c + 1, 1);
   }
+  if (c < n) chunk(c, 0);
   store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
 }
 template <int D>
@@ -725,12 +728,17 @@ struct TileF {
   static constexpr int UNITS = D / 4;
   static constexpr int PER = kChunkF32 * UNITS / THREADS;
   typedef f32x4 Regs[PER];
-  static __device__ __forceinline__ void load(Regs& r, const float* src, long ld, int live) {
+  static constexpr int STEP = THREADS / UNITS;
+  static __device__ __forceinline__ uint32_t offset(long ld) {
+    return ((uint32_t)(threadIdx.x / UNITS) * (uint32_t)ld + (threadIdx.x % UNITS) * 4) * 4;
+  }
+  static __device__ __forceinline__ void load(Regs& r, const float* src, long ld, uint32_t off, int live) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int u = i * THREADS + threadIdx.x, row = u / UNITS, c = u % UNITS;
-      r[i] = 0.f;
-      if (row < live) r[i] = *(const f32x4*)(src + row * ld + c * 4);
+      const int rows = min(max(live - STEP * i, 0), STEP);
+      const int bytes = __builtin_amdgcn_readfirstlane(rows ? (int)((uint32_t)((rows - 1) * ld + D) * 4) : 0);
+      r[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+          __builtin_amdgcn_make_buffer_rsrc((void*)(src + STEP * i * ld), 0, bytes, kBuffer), off, 0, 0));
     }
   }
   static __device__ __forceinline__ void put(float* tile, const Regs& r) {
@@ -775,11 +783,12 @@ __global__ __launch_bounds__(4 * D, 4) void linattn_sum_f32_kernel(Params p) {
   f32x4 S[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) S[t] = 0.f;
+  const uint32_t offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
   const int n = (w.live + kChunkF32 - 1) / kChunkF32;
   typename T::Regs ry, rz;
   auto fetch = [&](int c) {
-    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, w.live - c * kChunkF32);
-    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, w.live - c * kChunkF32);
+    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, offy, w.live - c * kChunkF32);
+    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, offz, w.live - c * kChunkF32);
   };
   if (n) fetch(0);
   for (int c = 0; c < n; ++c) {
@@ -831,13 +840,14 @@ __global__ __launch_bounds__(4 * D, 4) void linattn_walk_f32_kernel(Params p) {
     for (int t = 0; t < DT; ++t) S[t] = 0.f;
   }
   const bool keep_last = p.n_seg == 1 && ro.final_state;
+  const uint32_t offx = T::offset(ro.ldx), offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
   const int n = (w.live + kChunkF32 - 1) / kChunkF32;
   typename T::Regs rx, ry, rz;
   auto fetch = [&](int i) {
     const int c = rev ? n - 1 - i : i;
-    T::load(rx, x + (long)c * kChunkF32 * ro.ldx, ro.ldx, w.live - c * kChunkF32);
-    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, w.live - c * kChunkF32);
-    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, w.live - c * kChunkF32);
+    T::load(rx, x + (long)c * kChunkF32 * ro.ldx, ro.ldx, offx, w.live - c * kChunkF32);
+    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, offy, w.live - c * kChunkF32);
+    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, offz, w.live - c * kChunkF32);
   };
   if (n) fetch(0);
   pair_weights(&weights, w.g2, ro.a_pair, rev);
