@@ -244,9 +244,9 @@ struct Layout<32> {
   static __device__ __forceinline__ bf16x8 columns(uint32_t at, int t, int k) {
     typedef __attribute__((address_space(3))) s16x4* p16;
     // 8 rows, like 32 columns, flip bit 2 of the 16-byte unit
-    const uint32_t from = (at ^ ((t & 1) << 6)) + (t >> 1) * 8192 + k * 2048;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)from);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)((from ^ 64) + 1024));
+    const uint32_t even = at, odd = at ^ 64, past = (t >> 1) * 8192 + k * 2048;      // (two addresses, the rest an instruction's offset)
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)((t & 1 ? odd : even) + past));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p16)(uintptr_t)((t & 1 ? even : odd) + past + 1024));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   // per-row weights of a contraction step
