@@ -147,6 +147,38 @@ template <class V> __device__ __forceinline__ void leave(V* to, const V& v, bool
 // ---------------------------------------------------------------------------
 constexpr int kBuffer = 0x00027000;      // a buffer of 32-bit elements, no swizzle (word 3 of its description)
 
+// The chunks of a tensor's rows in the order of a walk.  A thread takes the units at `off`, `off` + `apart` ..
+struct Chunks {
+  const uint8_t* at;
+  long step;
+  uint32_t row, apart, off;      // bytes
+};
+template <class E, int STEP, int UNITS>
+__device__ __forceinline__ Chunks chunks_of(const E* rows, long ld, int chunk, int first, bool back) {
+  Chunks c;
+  const long bytes = (long)chunk * ld * (long)sizeof(E);
+  c.at = (const uint8_t*)rows + first * bytes;
+  c.step = back ? -bytes : bytes;
+  c.row = (uint32_t)ld * (uint32_t)sizeof(E);
+  c.apart = STEP * c.row;
+  c.off = (threadIdx.x / UNITS) * c.row + (threadIdx.x % UNITS) * 16;
+  return c;
+}
+// The next chunk, of which `live` rows are in the sequence: the others are out of the buffer's range, read nothing and count
+// as zero.  (A branch per row had every load in flight waited for, since their number was not known: sums of 2 x 4096 rows
+// of 32 heads on 8 60 us, 52 like this.)
+template <int N, int WIDTH, class V>
+__device__ __forceinline__ void next_chunk(V (&r)[N], Chunks& c, int live) {
+  const int bytes = __builtin_amdgcn_readfirstlane(live > 0 ? (int)((uint32_t)(live - 1) * c.row + WIDTH) : 0);
+  const auto buffer = __builtin_amdgcn_make_buffer_rsrc((void*)c.at, 0, bytes, kBuffer);
+  uint32_t off = c.off;
+  asm("" : "+v"(off) : "s"(bytes));        // (one register over the loop, not one for each load)
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    r[i] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(buffer, off + i * c.apart, 0, 0));
+  c.at += c.step;
+}
+
 template <int D>
 struct Tile {
   static constexpr int THREADS = 256;
@@ -164,17 +196,10 @@ struct Tile {
     const int c = threadIdx.x % UNITS;
     return (c >> 3) * 8192 + slab_off(threadIdx.x / UNITS, c & 7);
   }
-  // Rows from `live` on are out of the buffer's range, read nothing and count as zero.  (A branch per row had every load in
-  // flight waited for, since their number was not known: sums of 2 x 4096 rows of 32 heads on 8 60 us, 52 like this.)
-  static __device__ __forceinline__ void load(Regs& r, const bf16_t* src, long ld, uint32_t off, int live) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int rows = min(max(live - STEP * i, 0), STEP);
-      const int bytes = __builtin_amdgcn_readfirstlane(rows ? (int)((uint32_t)((rows - 1) * ld + D) * 2) : 0);
-      r[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-          __builtin_amdgcn_make_buffer_rsrc((void*)(src + STEP * i * ld), 0, bytes, kBuffer), off, 0, 0));
-    }
+  static __device__ __forceinline__ Chunks chunks(const bf16_t* rows, long ld, int first, bool back) {
+    return chunks_of<bf16_t, STEP, UNITS>(rows, ld, kChunk, first, back);
   }
+  static __device__ __forceinline__ void load(Regs& r, Chunks& c, int live) { next_chunk<PER, D * 2>(r, c, min(live, kChunk)); }
   static __device__ __forceinline__ void put(uint32_t at, const Regs& r) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) lds_put(at + i * STEP * 128, r[i]);
@@ -440,15 +465,15 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Para
   const bf16_t* y = rows_at<bf16_t>(ro.y, ro.ldy, ro.gy, p, w, D);
   const bf16_t* z = rows_at<bf16_t>(ro.z, ro.ldz, ro.gz, p, w, D);
   const uint32_t lds = lds_address(smem), unit = T::unit(), tr = L::tr(lane);
-  const uint32_t offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
   typename L::Acc S[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) S[t] = 0.f;
   const int n = (w.live + kChunk - 1) / kChunk;
   typename T::Regs ry[2], rz[2];       // two chunks on their way
+  Chunks cy = T::chunks(y, ro.ldy, 0, false), cz = T::chunks(z, ro.ldz, 0, false);
   auto fetch = [&](int c, int at) {
-    T::load(ry[at], y + (long)c * kChunk * ro.ldy, ro.ldy, offy, w.live - c * kChunk);
-    T::load(rz[at], z + (long)c * kChunk * ro.ldz, ro.ldz, offz, w.live - c * kChunk);
+    T::load(ry[at], cy, w.live - c * kChunk);
+    T::load(rz[at], cz, w.live - c * kChunk);
   };
   auto chunk = [&](int c, int at) {
     const int rows = min(kChunk, w.live - c * kChunk);
@@ -582,16 +607,18 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void linattn_walk_kernel(Par
   const bool keep_last = p.n_seg == 1 && ro.final_state;
   const uint32_t unit = T::unit(), tr = L::tr(lane), row = L::row(lane);
   const uint32_t unit_xy = L::CROSSED ? T::unit_crossed() : unit, tr_y = L::CROSSED ? L::tr_crossed(lane) : tr;
-  const uint32_t offx = T::offset(ro.ldx), offy = T::offset(ro.ldy), offz = T::offset(ro.ldz), offo = T::offset(ro.ldo);
+  const uint32_t offo = T::offset(ro.ldo);
   const long out_at = ((long)w.b * p.seq + w.s0) * ro.ldo + (long)(w.h / ro.go) * D;
 
   const int n = (w.live + kChunk - 1) / kChunk;
   typename T::Regs rx, ry, rz;
+  const int start = rev ? n - 1 : 0;
+  Chunks cx = T::chunks(x, ro.ldx, start, rev), cy = T::chunks(y, ro.ldy, start, rev), cz = T::chunks(z, ro.ldz, start, rev);
   auto fetch = [&](int i) {
-    const int c = rev ? n - 1 - i : i;
-    T::load(rx, x + (long)c * kChunk * ro.ldx, ro.ldx, offx, w.live - c * kChunk);
-    T::load(ry, y + (long)c * kChunk * ro.ldy, ro.ldy, offy, w.live - c * kChunk);
-    T::load(rz, z + (long)c * kChunk * ro.ldz, ro.ldz, offz, w.live - c * kChunk);
+    const int live = w.live - (rev ? n - 1 - i : i) * kChunk;
+    T::load(rx, cx, live);
+    T::load(ry, cy, live);
+    T::load(rz, cz, live);
   };
   if (n) fetch(0);
   pair_weights(weights, w.g2, ro.a_pair, rev);
@@ -728,18 +755,11 @@ struct TileF {
   static constexpr int UNITS = D / 4;
   static constexpr int PER = kChunkF32 * UNITS / THREADS;
   typedef f32x4 Regs[PER];
-  static constexpr int STEP = THREADS / UNITS;
-  static __device__ __forceinline__ uint32_t offset(long ld) {
-    return ((uint32_t)(threadIdx.x / UNITS) * (uint32_t)ld + (threadIdx.x % UNITS) * 4) * 4;
+  static __device__ __forceinline__ Chunks chunks(const float* rows, long ld, int first, bool back) {
+    return chunks_of<float, THREADS / UNITS, UNITS>(rows, ld, kChunkF32, first, back);
   }
-  static __device__ __forceinline__ void load(Regs& r, const float* src, long ld, uint32_t off, int live) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int rows = min(max(live - STEP * i, 0), STEP);
-      const int bytes = __builtin_amdgcn_readfirstlane(rows ? (int)((uint32_t)((rows - 1) * ld + D) * 4) : 0);
-      r[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-          __builtin_amdgcn_make_buffer_rsrc((void*)(src + STEP * i * ld), 0, bytes, kBuffer), off, 0, 0));
-    }
+  static __device__ __forceinline__ void load(Regs& r, Chunks& c, int live) {
+    next_chunk<PER, D * 4>(r, c, min(live, kChunkF32));
   }
   static __device__ __forceinline__ void put(float* tile, const Regs& r) {
 #pragma unroll
@@ -783,12 +803,12 @@ __global__ __launch_bounds__(4 * D, 4) void linattn_sum_f32_kernel(Params p) {
   f32x4 S[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) S[t] = 0.f;
-  const uint32_t offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
+  Chunks cy = T::chunks(y, ro.ldy, 0, false), cz = T::chunks(z, ro.ldz, 0, false);
   const int n = (w.live + kChunkF32 - 1) / kChunkF32;
   typename T::Regs ry, rz;
   auto fetch = [&](int c) {
-    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, offy, w.live - c * kChunkF32);
-    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, offz, w.live - c * kChunkF32);
+    T::load(ry, cy, w.live - c * kChunkF32);
+    T::load(rz, cz, w.live - c * kChunkF32);
   };
   if (n) fetch(0);
   for (int c = 0; c < n; ++c) {
@@ -840,14 +860,15 @@ __global__ __launch_bounds__(4 * D, 4) void linattn_walk_f32_kernel(Params p) {
     for (int t = 0; t < DT; ++t) S[t] = 0.f;
   }
   const bool keep_last = p.n_seg == 1 && ro.final_state;
-  const uint32_t offx = T::offset(ro.ldx), offy = T::offset(ro.ldy), offz = T::offset(ro.ldz);
   const int n = (w.live + kChunkF32 - 1) / kChunkF32;
+  const int start = rev ? n - 1 : 0;
+  Chunks cx = T::chunks(x, ro.ldx, start, rev), cy = T::chunks(y, ro.ldy, start, rev), cz = T::chunks(z, ro.ldz, start, rev);
   typename T::Regs rx, ry, rz;
   auto fetch = [&](int i) {
-    const int c = rev ? n - 1 - i : i;
-    T::load(rx, x + (long)c * kChunkF32 * ro.ldx, ro.ldx, offx, w.live - c * kChunkF32);
-    T::load(ry, y + (long)c * kChunkF32 * ro.ldy, ro.ldy, offy, w.live - c * kChunkF32);
-    T::load(rz, z + (long)c * kChunkF32 * ro.ldz, ro.ldz, offz, w.live - c * kChunkF32);
+    const int live = w.live - (rev ? n - 1 - i : i) * kChunkF32;
+    T::load(rx, cx, live);
+    T::load(ry, cy, live);
+    T::load(rz, cz, live);
   };
   if (n) fetch(0);
   pair_weights(&weights, w.g2, ro.a_pair, rev);
@@ -1094,7 +1115,7 @@ int check_tensor(const void* p, int64_t ld, int heads, int rows, const jpp_linat
   if (rows == 0) return JPP_OK;      // nothing of it is touched
   JPP_REQUIRE(p, "%s: null operand %s", who, name);
   JPP_REQUIRE(ld >= (int64_t)heads * a->head_dim, "%s: leading dimension of %s too small", who, name);
-  JPP_REQUIRE(ld < (1 << 26), "%s: leading dimension of %s too large", who, name);   // 16 rows in 32 bits of bytes
+  JPP_REQUIRE(ld < (1 << 25), "%s: leading dimension of %s too large", who, name);   // a chunk of rows in 32 bits of bytes
   JPP_REQUIRE(ld % unit == 0 && (uintptr_t)p % 16 == 0, "%s: %s must keep 16-byte alignment", who, name);
   return JPP_OK;
 }
