@@ -450,7 +450,7 @@ __device__ __forceinline__ const T* rows_at(const void* base, long ld, int group
 // ---------------------------------------------------------------------------
 // sums of the segments: parts[seg] = what the segment adds to the state that leaves it.  Rows are weighted to the
 // segment's end, so the accumulators are only added to.  Rows of two chunks ahead are on their way (16384 rows of 32 heads of 128:
-// 56 us, 4.8 TB/s; 69 with terms in three parts, the matrix cores' time).
+// 55 us, 4.9 TB/s; 68 with terms in three parts, the matrix cores' time).
 // ---------------------------------------------------------------------------
 template <int D, int PARTS>
 __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Params p) {
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
 // The state is held over a factor m that takes the decays, so that most chunks leave the accumulators alone: m falls by
 // lambda^rows a chunk, the new terms are divided by it, and below 2^-20 it is multiplied in.
 // PARTS: of the state's terms, see update_state.
-// 16384 rows of 32 heads of 128, forward: 125 us, 4.3 TB/s; gradients of 2 x 4096 rows of 32 heads: 185 us, there the phases of
+// 16384 rows of 32 heads of 128, forward: 122 us, 4.4 TB/s; gradients of 2 x 4096 rows of 32 heads on 8: 175 us, there the phases of
 // a chunk one after the other at two waves a SIMD (matrix cores 32 % of the time, vector instructions 30 %, LDS 27 %; no phase alone
 // is worth more than 42 us).
 // Three workgroups of heads of 64 fit a CU's LDS; registers for a fourth would be spilled ones (gradients of 2 x 4096 x 32
