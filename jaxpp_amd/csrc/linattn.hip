@@ -44,6 +44,7 @@ struct Role {
   int init_transposed;           // `init` holds the state's transpose
   int parts_transposed;          // and so does `parts`, another role's
   int out_f32;
+  int summed;                    // the results of a workgroup's two heads leave as their sum
   float a_pair, a_state, a_update;  // factors of the pair sum, of the state's part and of y^T z in the state
   const float* init;             // [batch, heads, D, D] or null (zero)
   float* final_state;            // [batch, heads, D, D] or null
@@ -57,6 +58,7 @@ struct Params {
   const int32_t* lens;
   int batch, seq, heads, group, n_seg, seg_rows;   // group: query heads per key head
   int past;            // results go past the caches
+  int pairs;           // two query heads to a workgroup of the walk
 };
 
 struct Place {
@@ -79,11 +81,12 @@ __device__ __forceinline__ int rows_of(const Params& p, int b) {
 }
 
 // Workgroups are dealt to the 8 XCDs in turn, each of which has an L2 of its own.  The roles and the query heads that
-// read the same rows of the same heads - n_roles x group workgroups - go to one XCD, one after the other, where their number
-// allows it.
+// read the same rows of the same heads go to one XCD, one after the other, where their number allows it.
+// H: query heads of a workgroup, 256 threads each.
+template <int H = 1>
 __device__ __forceinline__ Place place(const Params& p, int n_roles) {
   Place w;
-  const unsigned shared = n_roles * p.group, sets = gridDim.x / shared;
+  const unsigned shared = n_roles * (p.group / H), sets = gridDim.x / shared;
   unsigned set = blockIdx.x / shared, member = blockIdx.x % shared;
   if ((sets & 7) == 0) {
     const unsigned turn = blockIdx.x >> 3;
@@ -92,7 +95,7 @@ __device__ __forceinline__ Place place(const Params& p, int n_roles) {
   }
   const unsigned kv = p.heads / p.group;
   w.role = member % n_roles;
-  w.h = (set % kv) * p.group + member / n_roles;
+  w.h = (set % kv) * p.group + member / n_roles * H + (H > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0);
   set /= kv;
   w.seg = set % p.n_seg;
   w.b = set / p.n_seg;
@@ -141,6 +144,9 @@ template <class V> __device__ __forceinline__ void leave(V* to, const V& v, bool
   }
 }
 
+// a thread's place among the 256 of its head
+__device__ __forceinline__ int own_thread() { return threadIdx.x & 255; }
+
 // ---------------------------------------------------------------------------
 // bf16 tiles: [64][D] in LDS as D / 64 swizzled slabs, staged through registers (rows behind
 // the sequence's end are not read and count as zero)
@@ -161,7 +167,7 @@ __device__ __forceinline__ Chunks chunks_of(const E* rows, long ld, int chunk, i
   c.step = back ? -bytes : bytes;
   c.row = (uint32_t)ld * (uint32_t)sizeof(E);
   c.apart = STEP * c.row;
-  c.off = (threadIdx.x / UNITS) * c.row + (threadIdx.x % UNITS) * 16;
+  c.off = (threadIdx.x % (STEP * UNITS) / UNITS) * c.row + (threadIdx.x % UNITS) * 16;
   return c;
 }
 // The next chunk, of which `live` rows are in the sequence: the others are out of the buffer's range, read nothing and count
@@ -190,11 +196,11 @@ struct Tile {
 
   // the thread's byte offset from a chunk's first row, and its place in a tile
   static __device__ __forceinline__ uint32_t offset(long ld) {
-    return (uint32_t)((threadIdx.x / UNITS) * ld + (threadIdx.x % UNITS) * 8) * 2;
+    return (uint32_t)((own_thread() / UNITS) * ld + (own_thread() % UNITS) * 8) * 2;
   }
   static __device__ __forceinline__ uint32_t unit() {
-    const int c = threadIdx.x % UNITS;
-    return (c >> 3) * 8192 + slab_off(threadIdx.x / UNITS, c & 7);
+    const int c = own_thread() % UNITS;
+    return (c >> 3) * 8192 + slab_off(own_thread() / UNITS, c & 7);
   }
   static __device__ __forceinline__ Chunks chunks(const bf16_t* rows, long ld, int first, bool back) {
     return chunks_of<bf16_t, STEP, UNITS>(rows, ld, kChunk, first, back);
@@ -206,8 +212,8 @@ struct Tile {
   }
   // with the middle halves of every two units changed over: their units then hold elements 0 - 3 and 8 - 11, and 4 - 7 and 12 - 15
   static __device__ __forceinline__ uint32_t unit_crossed() {
-    const int c = threadIdx.x % UNITS;
-    return (c >> 3) * 8192 + slab_off(threadIdx.x / UNITS, c & 6) + (c & 1) * 8;
+    const int c = own_thread() % UNITS;
+    return (c >> 3) * 8192 + slab_off(own_thread() / UNITS, c & 6) + (c & 1) * 8;
   }
   static __device__ __forceinline__ void put_crossed(uint32_t at, const Regs& r) {
 #pragma unroll
@@ -369,14 +375,15 @@ struct Weights {
   float pair[128], up[kChunk], state[kChunk];
 };
 __device__ __forceinline__ void pair_weights(Weights* w, float g2, float a_pair, bool rev) {
-  for (int k = threadIdx.x; k < 128; k += blockDim.x) {
+  const int k = own_thread();
+  if (k < 128) {
     const int far = rev ? 64 - k : k - 64;
     w->pair[k] = far >= 0 ? a_pair * decay_pow(g2, far) : 0.f;
   }
 }
 __device__ __forceinline__ void row_weights(Weights* w, float g2, float a_update, float a_state, int rows, bool rev) {
-  if (threadIdx.x < kChunk) {
-    const int j = threadIdx.x, from_end = max(rows - 1 - j, 0);   // (rows behind the end are zero)
+  if (own_thread() < kChunk) {
+    const int j = own_thread(), from_end = max(rows - 1 - j, 0);   // (rows behind the end are zero)
     w->up[j] = a_update * decay_pow(g2, rev ? j + 1 : from_end);
     w->state[j] = a_state * decay_pow(g2, rev ? from_end : j + 1);
   }
@@ -574,21 +581,24 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
 template <int D>
 constexpr int walk_lds() { return 3 * Tile<D>::BYTES + 2 * 8192 + (int)sizeof(Weights); }
 
-template <int D, int PARTS>
-__global__ __launch_bounds__(256, D == 128 ? 2 : 3) void linattn_walk_kernel(Params p) {
+template <int D, int PARTS, int H>
+__global__ __launch_bounds__(256 * H, D == 128 ? 2 : 3) void linattn_walk_kernel(Params p) {
   using T = Tile<D>;
   using L = LayoutOf<D>;
   typedef typename L::Acc Acc;
   constexpr int W = D / 4, RT = kChunk / W, KC = kChunk / L::K;    // columns of a wave; row tiles and contraction steps of a chunk
-  extern __shared__ __align__(1024) uint8_t smem[];
+  static_assert(H == 1 || D == 128, "two heads: a unit of x for every four sums");
+  extern __shared__ __align__(1024) uint8_t all[];
+  const int half = H > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  uint8_t* const smem = all + half * walk_lds<D>();
   const uint32_t xtile = lds_address(smem);          // later the chunk's result
   const uint32_t ytile = xtile + T::BYTES, ztile = ytile + T::BYTES;
   const uint32_t ptile = ztile + T::BYTES;           // two parts of 8 KB, rows i, j in the accumulators' order
   Weights* const weights = (Weights*)(smem + 3 * T::BYTES + 2 * 8192);
   const uint32_t pair = lds_address(weights->pair), up = lds_address(weights->up), ofstate = lds_address(weights->state);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   const int line = L::line(lane);
-  const Place w = place(p, p.n_roles);
+  const Place w = place<H>(p, p.n_roles);
   const Role ro = p.role[w.role];
   const bool rev = ro.reverse;
   const bf16_t* x = rows_at<bf16_t>(ro.x, ro.ldx, ro.gx, p, w, D);
@@ -623,7 +633,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void linattn_walk_kernel(Par
   if (n) fetch(0);
   pair_weights(weights, w.g2, ro.a_pair, rev);
   // the tiles of pairs that never count stay zero
-  for (int k = threadIdx.x; k < 1024; k += T::THREADS) lds_put(ptile + k * 16, u32x4{0, 0, 0, 0});
+  for (int k = own_thread(); k < 1024; k += T::THREADS) lds_put(ptile + k * 16, u32x4{0, 0, 0, 0});
   __syncthreads();
   float m = 1.f;
   for (int i = 0; i < n; ++i) {
@@ -697,7 +707,27 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void linattn_walk_kernel(Par
     pairs(true, true);
     if (rev) pairs(false, true);
     else pairs(true, false);
-    if (ro.out_f32) {
+    Acc mine;
+    const bool summed = H == 2 && ro.summed;
+    if constexpr (H == 2) {
+      // Two heads' sum: each keeps the sums of one half of the rows and hands over the others, in the other's place of x, at the
+      // units that the taking thread overwrites with its next x.
+      if (summed) {
+        const uint32_t to = xtile + (half ? -walk_lds<D>() : walk_lds<D>()) + unit;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 give;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            give[e] = half ? o[0][4 * q + e] : o[1][4 * q + e];
+            mine[4 * q + e] = half ? o[1][4 * q + e] : o[0][4 * q + e];
+          }
+          lds_put(to + q * T::STEP * 128, give);
+        }
+      }
+    }
+    if (summed) {
+    } else if (ro.out_f32) {
       float* out = (float*)ro.out + out_at + (long)c * kChunk * ro.ldo + wave * W;
       int at = line;             // (addresses made here, not kept)
       asm volatile("" : "+v"(at));
@@ -726,19 +756,36 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void linattn_walk_kernel(Par
       update_state<D, PARTS>(S, ytile + tr_y, zf, up, lane);
     }
     __syncthreads();
-    if (!ro.out_f32) {
+    if constexpr (H == 2) {
+      const int at = half * W + line;
+      if (summed && at < rows) {
+        const long to = out_at + ((long)c * kChunk + at) * ro.ldo + wave * W;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 sum = lds_get<f32x4>(xtile + unit + q * T::STEP * 128);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] += mine[4 * q + e];
+          if (ro.out_f32)
+            *(f32x4*)((float*)ro.out + to + L::out_col(lane, q)) = sum;
+          else
+            *(u32x2*)((bf16_t*)ro.out + to + L::out_col(lane, q)) = u32x2{pack2(sum[0], sum[1]), pack2(sum[2], sum[3])};
+        }
+      }
+    }
+    if (!ro.out_f32 && !summed) {
       uint8_t* out = (uint8_t*)((bf16_t*)ro.out + out_at + (long)c * kChunk * ro.ldo);
 #pragma unroll
       for (int k = 0; k < T::PER; ++k)
         // (a unit that this wave overwrites with the next chunk's x)
-        if ((int)(threadIdx.x / T::UNITS) + T::STEP * k < rows)
+        if (own_thread() / T::UNITS + T::STEP * k < rows)
           leave((u32x4*)(out + 2 * T::STEP * k * ro.ldo + offo), lds_get<u32x4>(xtile + unit + k * T::STEP * 128), p.past);
     }
   }
   if (keep_last) store_state<D>(S, ro.final_state + bh * D * D, wave, lane);
   // rows behind the sequence's end
+  if (H == 2 && ro.summed && half) return;
   const int per = ro.out_f32 ? 4 : 8, units = D / per;
-  for (int k = threadIdx.x; k < (w.s1 - w.s0 - w.live) * units; k += T::THREADS) {
+  for (int k = own_thread(); k < (w.s1 - w.s0 - w.live) * units; k += T::THREADS) {
     const long at = ((long)w.b * p.seq + w.s0 + w.live + k / units) * ro.ldo + (long)(w.h / ro.go) * D + (k % units) * per;
     *(uint4*)((uint8_t*)ro.out + at * (ro.out_f32 ? 4 : 2)) = make_uint4(0, 0, 0, 0);
   }
@@ -1081,10 +1128,24 @@ int segment_rows(const jpp_linattn_args* a, int roles, int sums) {
   return (int)best;
 }
 
+// Two query heads of a group side by side in a workgroup, for gradients with heads of 128 (two of heads of 64 and their LDS leave
+// room for no second pair on a CU: 2 x 4096 rows of 32 heads on 8, 108 us, 137 with pairs).  The sum of their dk and dv is what leaves:
+// half the parts to write and to sum, none in groups of two (2 x 4096 rows of 32 heads on 16: 292 us, 232 with pairs; 32 on 8: 288 and
+// 274; 4 x 4096, 32 on 4: 496 and 455).  Not where the last of a few rounds leaves CUs with one workgroup, which a pair would not
+// (512 rows of 32 heads on 8: 8 sequences, a round and a half, 102 us, 114 with pairs; 11, a little over two, 162 and 173; 17, a
+// little over three, 238 and 231).
+bool pairs_of(const jpp_linattn_args* a, int segments) {
+  if (a->head_dim != 128 || a->dtype != JPP_DTYPE_BF16 || (a->n_heads / a->n_kv_heads) % 2) return false;
+  const int64_t walks = (int64_t)a->batch * a->n_heads * 3 * segments, slots = slots_of(128, false);
+  const int64_t last = walks % slots;
+  return walks > 3 * slots || last == 0 || last > slots / 2;
+}
+
 struct Split {
   int rows, n;
   size_t parts;        // bytes of one role's segment states
-  size_t groups;       // bytes of one gradient's query-head parts
+  int pairs;           // two query heads to a workgroup
+  size_t groups;       // bytes of one gradient's query-head parts (half of them are used with pairs)
 };
 Split split_of(const jpp_linattn_args* a, int roles) {
   Split s;
@@ -1093,6 +1154,7 @@ Split split_of(const jpp_linattn_args* a, int roles) {
   const size_t states = (size_t)a->batch * a->n_heads * a->head_dim * a->head_dim * 4;
   s.parts = s.n > 1 ? states * s.n : 0;
   s.groups = roles > 1 && a->n_kv_heads < a->n_heads ? (size_t)a->batch * a->seq * a->n_heads * a->head_dim * 4 : 0;
+  s.pairs = roles > 1 && pairs_of(a, s.n);
   return s;
 }
 
@@ -1129,6 +1191,23 @@ int check_state(const void* p, const char* who, const char* name) {
     if (int rc_ = (expr)) return rc_; \
   } while (0)
 
+template <int D, int H>
+int launch_walk(hipStream_t st, const Params& p) {
+  bool last = false;             // a state that is a result comes out of the walk
+  for (int i = 0; i < p.n_roles; ++i) last = last || (p.n_seg == 1 && p.role[i].final_state);
+  const dim3 grid((unsigned)((int64_t)p.batch * (p.heads / H) * p.n_roles * p.n_seg));
+  constexpr int lds = H * walk_lds<D>();
+  if (last) {
+    JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 3, H>, lds));
+    hipLaunchKernelGGL((linattn_walk_kernel<D, 3, H>), grid, dim3(256 * H), lds, st, p);
+  } else {
+    JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 2, H>, lds));
+    hipLaunchKernelGGL((linattn_walk_kernel<D, 2, H>), grid, dim3(256 * H), lds, st, p);
+  }
+  JPP_LAUNCH_CHECK();
+  return JPP_OK;
+}
+
 template <int D, bool F32>
 int launch(hipStream_t st, const Params& p) {
   const int64_t walks = (int64_t)p.batch * p.heads * p.n_roles, sums = (int64_t)p.batch * p.heads * p.n_sums;
@@ -1155,16 +1234,9 @@ int launch(hipStream_t st, const Params& p) {
   if constexpr (F32) {
     hipLaunchKernelGGL((linattn_walk_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(4 * D), 0, st, p);
   } else {
-    bool last = false;           // a state that is a result comes out of the walk
-    for (int i = 0; i < p.n_roles; ++i) last = last || (p.n_seg == 1 && p.role[i].final_state);
-    const dim3 grid((unsigned)(walks * p.n_seg));
-    if (last) {
-      JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 3>, walk_lds<D>()));
-      hipLaunchKernelGGL((linattn_walk_kernel<D, 3>), grid, dim3(256), walk_lds<D>(), st, p);
-    } else {
-      JPP_TRY(jpp_attn::set_smem(linattn_walk_kernel<D, 2>, walk_lds<D>()));
-      hipLaunchKernelGGL((linattn_walk_kernel<D, 2>), grid, dim3(256), walk_lds<D>(), st, p);
-    }
+    if constexpr (D == 128)
+      if (p.pairs) return launch_walk<D, 2>(st, p);
+    return launch_walk<D, 1>(st, p);
   }
   JPP_LAUNCH_CHECK();
   return JPP_OK;
@@ -1187,6 +1259,7 @@ Params params_of(const jpp_linattn_args* a, const Split& s) {
   // of 32 heads of 128, 67 MB: 83 -> 72 us).
   p.past = (int64_t)a->batch * a->seq * a->n_heads * a->head_dim >= (int64_t)16 << 20;
   p.n_seg = s.n;
+  p.pairs = s.pairs;
   p.seg_rows = s.rows;
   return p;
 }
@@ -1221,7 +1294,7 @@ extern "C" int jpp_linattn_fwd(void* stream, const jpp_linattn_args* a) {
   const int group = a->n_heads / a->n_kv_heads;
   Params p = params_of(a, s);
   p.n_roles = p.n_sums = 1;
-  p.role[0] = {a->q, a->k, a->v, a->o, a->ldq, a->ldk, a->ldv, a->ldo, 1, group, group, 1, 0, 0, 0, 0,
+  p.role[0] = {a->q, a->k, a->v, a->o, a->ldq, a->ldk, a->ldv, a->ldo, 1, group, group, 1, 0, 0, 0, 0, 0,
                a->scale, a->scale, 1.f, a->state_in, a->state_out, (float*)a->workspace};
   const double es = a->dtype == JPP_DTYPE_F32 ? 4 : 2;
   ProbeScope probe((hipStream_t)stream, "linattn_fwd", 2 * flops_of(a),
@@ -1254,22 +1327,23 @@ extern "C" int jpp_linattn_bwd(void* stream, const jpp_linattn_args* a) {
   JPP_REQUIRE(s.parts + s.groups == 0 || a->workspace, "%s: workspace of %zu bytes wanted", who, 2 * s.parts + 2 * s.groups);
   JPP_TRY(check_state(a->workspace, who, "workspace"));
   const int group = a->n_heads / a->n_kv_heads, f32 = a->dtype == JPP_DTYPE_F32;
-  const long wide = (long)a->n_heads * a->head_dim;
+  const int each = s.pairs ? 2 : 1;
+  const long wide = (long)(a->n_heads / each) * a->head_dim;
   uint8_t* ws = (uint8_t*)a->workspace;
   float* const s_parts = (float*)ws;
   float* const u_parts = (float*)(ws + s.parts);
   float* const dk_parts = (float*)(ws + 2 * s.parts);
   float* const dv_parts = (float*)(ws + 2 * s.parts + s.groups);
-  const bool shared = s.groups != 0;
+  const bool shared = s.groups && group > each;      // query heads' parts are left to sum
   Params p = params_of(a, s);
   p.n_roles = 3;
   p.n_sums = 2;
-  p.role[0] = {a->d_o, a->v, a->k, a->dq, a->lddo, a->ldv, a->ldk, a->lddq, 1, group, group, 1, 0, 1, 0, 0,
+  p.role[0] = {a->d_o, a->v, a->k, a->dq, a->lddo, a->ldv, a->ldk, a->lddq, 1, group, group, 1, 0, 1, 0, 0, 0,
                a->scale, a->scale, 1.f, a->state_in, nullptr, s_parts};
   p.role[1] = {a->k, a->q, a->d_o, shared ? (void*)dv_parts : a->dv, a->ldk, a->ldq, a->lddo, shared ? wide : (long)a->lddv,
-               group, 1, 1, 1, 1, 0, 0, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, a->d_state_in, u_parts};
+               group, 1, 1, each, 1, 0, 0, shared && !f32, s.pairs, a->scale, 1.f, a->scale, a->d_state_out, a->d_state_in, u_parts};
   p.role[2] = {a->v, a->d_o, a->q, shared ? (void*)dk_parts : a->dk, a->ldv, a->lddo, a->ldq, shared ? wide : (long)a->lddk,
-               group, 1, 1, 1, 1, 1, 1, shared && !f32, a->scale, 1.f, a->scale, a->d_state_out, nullptr, u_parts};
+               group, 1, 1, each, 1, 1, 1, shared && !f32, s.pairs, a->scale, 1.f, a->scale, a->d_state_out, nullptr, u_parts};
   hipStream_t st = (hipStream_t)stream;
   const double es = f32 ? 4 : 2;
   ProbeScope probe(st, "linattn_bwd", 5 * flops_of(a),
@@ -1281,10 +1355,10 @@ extern "C" int jpp_linattn_bwd(void* stream, const jpp_linattn_args* a) {
     const dim3 grid((unsigned)std::min<long>((units + 255) / 256, 1 << 20), 2);
     if (f32)
       hipLaunchKernelGGL((linattn_group_sum_kernel<float>), grid, dim3(256), 0, st, dk_parts, dv_parts, (float*)a->dk,
-                         (float*)a->dv, a->lddk, a->lddv, rows, a->n_kv_heads, group, a->head_dim);
+                         (float*)a->dv, a->lddk, a->lddv, rows, a->n_kv_heads, group / each, a->head_dim);
     else
       hipLaunchKernelGGL((linattn_group_sum_kernel<bf16_t>), grid, dim3(256), 0, st, dk_parts, dv_parts, (bf16_t*)a->dk,
-                         (bf16_t*)a->dv, a->lddk, a->lddv, rows, a->n_kv_heads, group, a->head_dim);
+                         (bf16_t*)a->dv, a->lddk, a->lddv, rows, a->n_kv_heads, group / each, a->head_dim);
     JPP_LAUNCH_CHECK();
   }
   return JPP_OK;

@@ -326,3 +326,11 @@ def test_results_of_more_than_the_caches(heads, dim, seq):
     want, size = O.linattn_bwd(q, k, v, d_o, *args, None, None, None), O.linattn_bwd(*sizes, *args, None, None, None)
     for name, got, w, m in zip(("dq", "dk", "dv"), p.backward(), want, size):
         _close(got[:, :, pick], w, m, False, name)
+
+
+@pytest.mark.parametrize("batch,seq,heads,kv,lens", [(3, 131, 32, 16, None), (3, 131, 32, 8, [131, 0, 70]), (3, 64, 32, 2, [1, 64, 33]),
+                                                     (1, 900, 16, 8, None), (1, 900, 16, 4, [777])])
+def test_heads_in_pairs(batch, seq, heads, kv, lens):
+    """Gradients of shared heads of 128 with workgroups for more than half of the device: two query heads to one."""
+    Problem(batch, seq, heads, kv, 128, lens=lens, seed=7).check_backward()
+    Problem(batch, seq, heads, kv, 128, lens=lens, states=False, seed=8).check_backward()
