@@ -232,3 +232,49 @@ def test_repeats_are_bit_identical_on_another_stream_and_in_a_graph():
 def test_gradients_of_more_than_the_caches(rows, cols, f32):
     """Gradients of 16 M elements and more are stored past the caches; a workgroup has several rows."""
     Problem(rows, cols, f32, gate_rows=rows // 2, seed=6).check_backward()
+
+
+def test_more_elements_than_31_bits_count():
+    """A few rows of tensors of 4 GiB and more are given and looked at."""
+    rows, cols = (1 << 18) + 8, 8192
+    pick = [0, 77, (1 << 18) - 1, (1 << 18) + 3, rows - 1]
+    p = Problem(len(pick), cols, seed=10)
+    dev = p._weights()
+    w = {n: _ptr(v) for n, v in dev.items()}
+    big = {n: rt.DeviceBuffer(2 * rows * cols) for n in ("x", "b", "h", "y", "dx", "db")}
+    stat = {n: rt.DeviceBuffer(4 * rows) for n in ("rstd_post", "rstd_pre")}
+
+    def put(buf, a):
+        for i, r in enumerate(pick):
+            buf.upload(rt.to_bf16_bits(a[i]), 2 * r * cols)
+
+    def get(buf):
+        return np.stack([rt.from_bf16_bits(buf.download(np.uint16, (cols,), 2 * r * cols)) for r in pick])
+
+    put(big["x"], p.x)
+    put(big["b"], p.b)
+    rt.block_join_fwd(big["x"].ptr, big["b"].ptr, big["h"].ptr, rows, cols, y=big["y"].ptr, rstd_post=stat["rstd_post"].ptr,
+                      rstd_pre=stat["rstd_pre"].ptr, alpha=p.alpha, eps=EPS, **w)
+    rt.sync()
+    want = O.block_join(p.x, p.b, p.gamma_post, None, 0, p.gamma_pre, p.alpha, EPS)
+    size = p.alpha * np.abs(p.x) + np.abs(p.b) * want["rstd_post"][:, None] * np.abs(p.gamma_post)
+    grow = np.sqrt(np.mean(size ** 2, 1) / (np.mean(want["h"] ** 2, 1) + EPS))[:, None]
+    _close(get(big["h"]), want["h"], size, False, "h")
+    _close(get(big["y"]), want["y"], (size + np.abs(want["h"]) * grow) * want["rstd_pre"][:, None] * np.abs(p.gamma_pre), False, "y")
+
+    put(big["h"], p.h)
+    put(big["x"], p.dh)
+    put(big["y"], p.dy)
+    r_post, r_pre = ((1 / np.sqrt(np.mean(a.astype(np.float64) ** 2, 1) + EPS)).astype(np.float32) for a in (p.b, p.h))
+    for i, r in enumerate(pick):
+        stat["rstd_post"].upload(r_post[i:i + 1], 4 * r)
+        stat["rstd_pre"].upload(r_pre[i:i + 1], 4 * r)
+    rt.block_join_bwd(big["h"].ptr, big["b"].ptr, big["x"].ptr, big["y"].ptr, big["dx"].ptr, big["db"].ptr, rows, cols,
+                      rstd_post=stat["rstd_post"].ptr, rstd_pre=stat["rstd_pre"].ptr, alpha=p.alpha, **w)
+    rt.sync()
+    want = O.block_join_bwd(p.h, p.b, p.dh, p.dy, p.gamma_post, None, 0, p.gamma_pre, r_post, r_pre, p.alpha)
+    hat, t = np.abs(p.h * r_pre[:, None].astype(np.float64)), np.abs(p.dy * p.gamma_pre)
+    total = np.abs(p.dh) + r_pre[:, None] * (t + hat * np.mean(t * hat, 1, keepdims=True))
+    n, u = np.abs(p.b) * r_post[:, None], total * np.abs(p.gamma_post)
+    _close(get(big["dx"]), want["dx"], p.alpha * total, False, "dx")
+    _close(get(big["db"]), want["db"], r_post[:, None] * (u + n * np.mean(u * n, 1, keepdims=True)), False, "db")

@@ -204,3 +204,25 @@ def test_repeats_on_another_stream_and_in_a_graph(rows, vocab):
         for b in (row_loss, loss, dz, ws):
             b.zero()
         rt.sync()
+
+
+def test_rows_far_apart():
+    """More than 2^31 elements from the first row to the last."""
+    rows, vocab, ld = 9, 1001, 1 << 28
+    p = Problem(rows, vocab, 12)
+    z = rt.DeviceBuffer(2 * ((rows - 1) * ld + vocab))
+    bits = rt.to_bf16_bits(p.z)
+    for r in range(rows):
+        z.upload(bits[r], 2 * r * ld)
+    ids, teacher, w = (rt.DeviceBuffer.from_numpy(a) for a in (p.ids, p.teacher, p.w))
+    row_loss = rt.DeviceBuffer(4 * rows)
+    p.ld = p.ldd = vocab
+    for workspace in (False, True):       # in place, and before it the losses alone
+        ws = rt.DeviceBuffer(rt.load().jpp_workspace_bytes(8, rows, 0, 0))
+        rt.distill_loss(z.ptr, ids.ptr, teacher.ptr, rows, vocab, 12, ld, row_loss.ptr, dlogits=z.ptr if workspace else None, ldd=ld,
+                        weight=w.ptr, temperature=p.t, scale=p.scale, workspace=ws.ptr if workspace else None)
+        rt.sync()
+        row = row_loss.download(np.float32, (rows,))
+        got = np.stack([rt.from_bf16_bits(z.download(np.uint16, (vocab,), 2 * r * ld)) for r in range(rows)])
+        p.run = lambda: (row, p.scale * float(row.sum(dtype=np.float64)), got if workspace else None)
+        p.check()

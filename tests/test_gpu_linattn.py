@@ -334,3 +334,32 @@ def test_heads_in_pairs(batch, seq, heads, kv, lens):
     """Gradients of shared heads of 128 with workgroups for more than half of the device: two query heads to one."""
     Problem(batch, seq, heads, kv, 128, lens=lens, seed=7).check_backward()
     Problem(batch, seq, heads, kv, 128, lens=lens, states=False, seed=8).check_backward()
+
+
+@pytest.mark.parametrize("f32,dim", [(False, 128), (False, 64), (True, 128)])
+def test_rows_far_apart(f32, dim):
+    """The largest leading dimension: a chunk's rows span almost 4 GiB, the tensors 10 and 20."""
+    seq, ld, es = 150, (1 << 25) - 8, 4 if f32 else 2
+    p = Problem(1, seq, 1, 1, dim, f32, states=False, seed=9)
+    names = ("q", "k", "v", "d_o", "o", "dq", "dk", "dv")
+    buf = rt.DeviceBuffer(es * ((seq - 1) * ld + len(names) * dim))
+    ptr = {n: buf.ptr + es * dim * i for i, n in enumerate(names)}
+    row = np.full((seq, len(names), dim), 7.0, np.float32)
+    for i, n in enumerate(names[:4]):
+        row[:, i] = getattr(p, n)[0, :, 0]
+    row = row if f32 else rt.to_bf16_bits(row)
+    for t in range(seq):
+        buf.upload(row[t], es * t * ld)
+    decay = _up(p.decay)
+    ws = [rt.DeviceBuffer(rt.linattn_workspace(1, seq, 1, 1, dim, back, f32) + 16) for back in (False, True)]
+    rt.linattn_fwd(ptr["q"], ptr["k"], ptr["v"], ptr["o"], decay.ptr, ld, ld, ld, ld, workspace=ws[0].ptr, **p.sizes)
+    rt.linattn_bwd(ptr["q"], ptr["k"], ptr["v"], ptr["d_o"], ptr["dq"], ptr["dk"], ptr["dv"], decay.ptr, ld, ld, ld, ld, ld, ld, ld,
+                   workspace=ws[1].ptr, **p.sizes)
+    rt.sync()
+    got = np.stack([buf.download(np.float32 if f32 else np.uint16, (len(names), dim), es * t * ld) for t in range(seq)])
+    got = got if f32 else rt.from_bf16_bits(got)
+    args, sizes = (p.decay, p.sizes["scale"]), [np.abs(a) for a in (p.q, p.k, p.v, p.d_o)]
+    want = (O.linattn(p.q, p.k, p.v, *args)[0], *O.linattn_bwd(p.q, p.k, p.v, p.d_o, *args)[:3])
+    size = (O.linattn(*sizes[:3], *args)[0], *O.linattn_bwd(*sizes, *args)[:3])
+    for i, name in enumerate(names[4:]):
+        _close(got[None, :, None, 4 + i], want[i], size[i], f32, name)
