@@ -5,7 +5,7 @@
 //
 // HBM-bound: the logits are read, their gradient is written.  One workgroup per row: the running maximum and sum of the
 // softmax in one pass over the row, q in a second, which finds the first units in registers and the others in the
-// caches.  Where rows are fewer than CUs they are cut into pieces: a launch that takes each piece's maximum and sum, and one
+// caches.  Where rows are few they are cut into pieces: a launch that takes each piece's maximum and sum, and one
 // that joins them and writes.  The few listed places are written last, each by one thread, so no result depends on timing.
 // 4096 x 128256 bf16: 415 us, 5.1 TB/s.
 #include <math.h>
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(T, WAVES) void distill_kernel(DistillParams p) {
 // the last the listed part of the loss with its reference.
 // ---------------------------------------------------------------------------
 constexpr int kPieceThreads = 256, kPieceHeld = 8;
-constexpr int kPieces = 62, kPieceRows = 256;
+constexpr int kPieces = 62;
 
 template <class E>
 __global__ __launch_bounds__(kPieceThreads) void distill_scan_kernel(DistillParams p, float2* ws, int per) {
@@ -515,9 +515,11 @@ extern "C" int jpp_distill_loss(void* stream, const jpp_distill_args* a) {
   const int units = (int)(a->vocab / (f32 ? 4 : 8));
   // (5 rows of 50021 f32: 3.6 + 5.5 us in pieces of two units a thread, 4.0 + 6.9 of eight; 128 rows of 128256 bf16: 15.8 + 21.6 and
   // 8.5 + 18.7)
+  // In pieces as long as one workgroup a row leaves most of the device idle (128256 wide, whole rows and pieces: 16 rows f32 21.9 and
+  // 13.1 us, 48 rows 22.1 and 22.7, 96 rows 27.4 and 36.6; bf16 16 rows 21.7 and 11.3, 128 rows 23.3 and 23.4).
   const int per = std::max(kPieceThreads * (a->rows <= 16 ? 2 : kPieceHeld), (units + kPieces - 1) / kPieces);
   const int pieces = (units + per - 1) / per;
-  if (a->workspace && a->rows < kPieceRows && pieces > 1)
+  if (a->workspace && a->rows < (f32 ? 48 : 128) && pieces > 1)
     return f32 ? launch_pieces<float>(st, p, (int)a->rows, a->loss, (float2*)a->workspace, pieces, per)
                : launch_pieces<bf16_t>(st, p, (int)a->rows, a->loss, (float2*)a->workspace, pieces, per);
   if (f32) launch<float>(st, p, a->rows);
