@@ -10,6 +10,7 @@ from __future__ import annotations
 import atexit
 import ctypes as C
 import os
+import struct
 from typing import Iterable
 
 import numpy as np
@@ -113,6 +114,17 @@ class DistillArgs(C.Structure):
                 ("ld", C.c_int64),
                 ("ldd", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int64), ("k", C.c_int),
                 ("temperature", C.c_float), ("scale", C.c_float), ("dtype", C.c_int)]
+
+
+def _packer(args):
+    """`args` as bytes, for calls of a few microseconds: a Structure takes three times as long to fill."""
+    codes = {C.c_void_p: "P", C.c_int64: "q", C.c_int: "i", C.c_float: "f"}
+    layout = struct.Struct("".join(codes[t] for _, t in args._fields_) + "0P")
+    assert layout.size == C.sizeof(args)
+    return layout.pack
+
+
+_pack_linattn, _pack_join, _pack_distill = _packer(LinattnArgs), _packer(JoinArgs), _packer(DistillArgs)
 
 
 class StageDesc(C.Structure):
@@ -278,6 +290,10 @@ def load():
     for name in ("fwd", "bwd"):
         getattr(lib, "jpp_block_join_" + name).argtypes = [C.c_void_p, C.POINTER(JoinArgs)]
     lib.jpp_distill_loss.argtypes = [C.c_void_p, C.POINTER(DistillArgs)]
+    lib.packed = {}
+    for name in ("linattn_fwd", "linattn_bwd", "linattn_step", "block_join_fwd", "block_join_bwd", "distill_loss"):
+        lib.packed[name] = lib["jpp_" + name]         # (a function object of its own)
+        lib.packed[name].argtypes = [C.c_void_p, C.c_char_p]
     lib.jpp_stage_create.argtypes = [C.POINTER(StageDesc), C.POINTER(C.c_void_p)]
     lib.jpp_stage_destroy.argtypes = [C.c_void_p]
     lib.jpp_stage_n_params.argtypes = [C.c_void_p]
@@ -662,51 +678,53 @@ def linattn_workspace(batch, seq, n_heads, n_kv_heads, head_dim, backward=False,
 def linattn_fwd(q, k, v, o, decay, ldq, ldk, ldv, ldo, batch, seq, n_heads, n_kv_heads, head_dim, scale, state_in=None,
                 state_out=None, lens=None, workspace=None, f32=False, stream=None):
     """Linear attention with a decay for each head (jpp_linattn_fwd)."""
-    check(load().jpp_linattn_fwd(stream, LinattnArgs(
-        q, k, v, o, None, None, None, None, decay, state_in, state_out, None, None, lens, workspace, ldq, ldk, ldv, ldo,
-        0, 0, 0, 0, batch, seq, n_heads, n_kv_heads, head_dim, scale, f32)))
+    check(load().packed["linattn_fwd"](stream, _pack_linattn(
+        q or 0, k or 0, v or 0, o or 0, 0, 0, 0, 0, decay or 0, state_in or 0, state_out or 0, 0, 0, lens or 0,
+        workspace or 0, ldq, ldk, ldv, ldo, 0, 0, 0, 0, batch, seq, n_heads, n_kv_heads, head_dim, scale, f32)))
 
 
 def linattn_bwd(q, k, v, d_o, dq, dk, dv, decay, ldq, ldk, ldv, lddo, lddq, lddk, lddv, batch, seq, n_heads, n_kv_heads,
                 head_dim, scale, state_in=None, d_state_out=None, d_state_in=None, lens=None, workspace=None, f32=False,
                 stream=None):
     """Its gradients (jpp_linattn_bwd)."""
-    check(load().jpp_linattn_bwd(stream, LinattnArgs(
-        q, k, v, None, d_o, dq, dk, dv, decay, state_in, None, d_state_out, d_state_in, lens, workspace, ldq, ldk, ldv, 0,
-        lddo, lddq, lddk, lddv, batch, seq, n_heads, n_kv_heads, head_dim, scale, f32)))
+    check(load().packed["linattn_bwd"](stream, _pack_linattn(
+        q or 0, k or 0, v or 0, 0, d_o or 0, dq or 0, dk or 0, dv or 0, decay or 0, state_in or 0, 0,
+        d_state_out or 0, d_state_in or 0, lens or 0, workspace or 0, ldq, ldk, ldv, 0, lddo, lddq, lddk, lddv, batch,
+        seq, n_heads, n_kv_heads, head_dim, scale, f32)))
 
 
 def linattn_step(q, k, v, o, decay, state_in, state_out, ldq, ldk, ldv, ldo, batch, n_heads, n_kv_heads, head_dim, scale,
                  f32=False, stream=None):
     """One token per sequence (jpp_linattn_step); `state_out` may be `state_in`."""
-    check(load().jpp_linattn_step(stream, LinattnArgs(
-        q, k, v, o, None, None, None, None, decay, state_in, state_out, None, None, None, None, ldq, ldk, ldv, ldo,
-        0, 0, 0, 0, batch, 0, n_heads, n_kv_heads, head_dim, scale, f32)))
+    check(load().packed["linattn_step"](stream, _pack_linattn(
+        q or 0, k or 0, v or 0, o or 0, 0, 0, 0, 0, decay or 0, state_in or 0, state_out or 0, 0, 0, 0, 0, ldq, ldk,
+        ldv, ldo, 0, 0, 0, 0, batch, 0, n_heads, n_kv_heads, head_dim, scale, f32)))
 
 
 def block_join_fwd(x, b, h, rows, cols, y=None, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None, rstd_post=None,
                    rstd_pre=None, alpha=1.0, eps=1e-6, f32=False, stream=None):
     """A block's output joined to the residual stream: norm, gate, residual scale, next norm (jpp_block_join_fwd)."""
-    check(load().jpp_block_join_fwd(stream, JoinArgs(
-        x, b, gamma_post, gate, gamma_pre, h, y, rstd_post, rstd_pre, None, None, None, None, None, None, None, None, rows,
-        cols, gate_rows, alpha, eps, 0, f32)))
+    check(load().packed["block_join_fwd"](stream, _pack_join(
+        x or 0, b or 0, gamma_post or 0, gate or 0, gamma_pre or 0, h or 0, y or 0, rstd_post or 0, rstd_pre or 0, 0,
+        0, 0, 0, 0, 0, 0, 0, rows, cols, gate_rows, alpha, eps, 0, f32)))
 
 
 def block_join_bwd(h, b, dh, dy, dx, db, rows, cols, gamma_post=None, gate=None, gate_rows=0, gamma_pre=None,
                    rstd_post=None, rstd_pre=None, dgamma_post=None, dgate=None, dgamma_pre=None, workspace=None,
                    alpha=1.0, accumulate=True, f32=False, stream=None):
     """Its gradients (jpp_block_join_bwd); the sums over rows are added to what is there if `accumulate`."""
-    check(load().jpp_block_join_bwd(stream, JoinArgs(
-        None, b, gamma_post, gate, gamma_pre, h, None, rstd_post, rstd_pre, dh, dy, dx, db, dgamma_post, dgate, dgamma_pre,
-        workspace, rows, cols, gate_rows, alpha, 0.0, accumulate, f32)))
+    check(load().packed["block_join_bwd"](stream, _pack_join(
+        0, b or 0, gamma_post or 0, gate or 0, gamma_pre or 0, h or 0, 0, rstd_post or 0, rstd_pre or 0, dh or 0,
+        dy or 0, dx or 0, db or 0, dgamma_post or 0, dgate or 0, dgamma_pre or 0, workspace or 0, rows, cols,
+        gate_rows, alpha, 0.0, accumulate, f32)))
 
 
 def distill_loss(logits, ids, teacher, rows, vocab, k, ld, row_loss, loss=None, dlogits=None, ldd=0, weight=None,
                  temperature=1.0, scale=1.0, workspace=None, f32=False, stream=None):
     """Loss and gradient of logits against a teacher's top logits (jpp_distill_loss)."""
-    check(load().jpp_distill_loss(stream, DistillArgs(
-        logits, ids, teacher, weight, row_loss, loss, dlogits, workspace, ld, ldd, rows, vocab, k, temperature, scale,
-        f32)))
+    check(load().packed["distill_loss"](stream, _pack_distill(
+        logits or 0, ids or 0, teacher or 0, weight or 0, row_loss or 0, loss or 0, dlogits or 0, workspace or 0, ld,
+        ldd, rows, vocab, k, temperature, scale, f32)))
 
 
 # Elements of tensors that travel in one call, or one larger tensor (of a layer's results, the layer): what bounds the
