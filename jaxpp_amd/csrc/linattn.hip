@@ -456,8 +456,11 @@ __device__ __forceinline__ const T* rows_at(const void* base, long ld, int group
 
 // ---------------------------------------------------------------------------
 // sums of the segments: parts[seg] = what the segment adds to the state that leaves it.  Rows are weighted to the
-// segment's end, so the accumulators are only added to.  Rows of two chunks ahead are on their way (16384 rows of 32 heads of 128:
-// 55 us, 4.9 TB/s; 68 with terms in three parts, the matrix cores' time).
+// segment's end, so the accumulators are only added to.  In a forward with heads of 64 this goes from the end, so that the walk finds
+// the rows it begins with still in the caches (16384 rows of 64 heads 178 us, 164 like this; 8192 83.5 and 81.2; with heads of
+// 128, whose walk waits less for memory, 16384 rows of 24 137 and 139; gradients walk both ways, 2 x 4096 of 32 heads of 128 216
+// and 219).  Rows of two chunks ahead are on their way (16384 rows of 32 heads of 128: 55 us, 4.9 TB/s; 68 with terms in three
+// parts, the matrix cores' time).
 // ---------------------------------------------------------------------------
 template <int D, int PARTS>
 __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Params p) {
@@ -477,12 +480,15 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Para
   for (int t = 0; t < 4; ++t) S[t] = 0.f;
   const int n = (w.live + kChunk - 1) / kChunk;
   typename T::Regs ry[2], rz[2];       // two chunks on their way
-  Chunks cy = T::chunks(y, ro.ldy, 0, false), cz = T::chunks(z, ro.ldz, 0, false);
-  auto fetch = [&](int c, int at) {
-    T::load(ry[at], cy, w.live - c * kChunk);
-    T::load(rz[at], cz, w.live - c * kChunk);
+  const bool back = D == 64 && p.n_roles == 1;
+  Chunks cy = T::chunks(y, ro.ldy, back ? n - 1 : 0, back), cz = T::chunks(z, ro.ldz, back ? n - 1 : 0, back);
+  auto fetch = [&](int i, int at) {
+    const int live = i < n ? w.live - (back ? n - 1 - i : i) * kChunk : 0;
+    T::load(ry[at], cy, live);
+    T::load(rz[at], cz, live);
   };
-  auto chunk = [&](int c, int at) {
+  auto chunk = [&](int i, int at) {
+    const int c = back ? n - 1 - i : i;
     const int rows = min(kChunk, w.live - c * kChunk);
     const uint32_t ytile = lds + at * (2 * T::BYTES + kChunk * 4), ztile = ytile + T::BYTES, up = ztile + T::BYTES;
     // rows between this chunk and the end that the state leaves by
@@ -494,7 +500,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Para
     T::put(ytile + unit, ry[at]);
     T::put(ztile + unit, rz[at]);
     __syncthreads();       // (and nobody is still reading the stage that the next chunk fills)
-    fetch(c + 2, at);      // (behind the last one: nothing)
+    fetch(i + 2, at);      // (behind the last one: nothing)
     bf16x8 zf[kChunk / L::K];
 #pragma unroll
     for (int k = 0; k < kChunk / L::K; ++k) zf[k] = L::columns(ztile + tr, wave, k);
@@ -503,12 +509,12 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void linattn_sum_kernel(Para
   fetch(0, 0);
   asm volatile("" ::: "memory");       // (in this order, as in the loop: what is waited for is counted)
   fetch(1, 1);
-  int c = 0;
-  for (; c + 1 < n; c += 2) {
-    chunk(c, 0);
-    chunk(c + 1, 1);
+  int i = 0;
+  for (; i + 1 < n; i += 2) {
+    chunk(i, 0);
+    chunk(i + 1, 1);
   }
-  if (c < n) chunk(c, 0);
+  if (i < n) chunk(i, 0);
   store_state<D>(S, ro.parts + (((long)w.b * p.heads + w.h) * p.n_seg + w.seg) * D * D, wave, lane);
 }
 template <int D>
