@@ -18,8 +18,8 @@
 // A workgroup walks a segment of a sequence in chunks of rows (bf16: 64, f32: 32): within a chunk the pairs
 // are products of tiles, between chunks the state is carried in f32 accumulators, each wave some columns of it.
 // Where batch x heads give too few workgroups, a sequence is cut into segments: a first launch sums
-// every segment's y^T z, a second carries them over the segments (small), and the walk starts each segment from
-// its state.
+// every segment's y^T z, and a walk starts from its segment's state: the sums of the segments before it, added up by the walk
+// where those are few, by a launch that carries them over the segments where they are many.
 #include <math.h>
 
 #include <algorithm>
@@ -59,6 +59,7 @@ struct Params {
   int batch, seq, heads, group, n_seg, seg_rows;   // group: query heads per key head
   int past;            // results go past the caches
   int pairs;           // two query heads to a workgroup of the walk
+  int carried;         // a launch of its own has made the segments' sums states
 };
 
 struct Place {
@@ -449,6 +450,32 @@ __device__ __forceinline__ void store_state(const typename Layout<W>::Acc (&S)[D
     for (int r = 0; r < W * W / 64; ++r) dst[(t * W + L::row_of(lane, r)) * D + col] = S[t][r];
 }
 
+// The state that a walk starts from: as carried there, or what entered the sequence and the sums of the segments before this one.
+template <int D, int W = D / 4>
+__device__ __forceinline__ void entering_state(typename Layout<W>::Acc (&S)[D / W], const Params& p, const Role& ro, const Place& w,
+                                               int wave, int lane) {
+  const long bh = (long)w.b * p.heads + w.h;
+  const float* parts = ro.parts + bh * p.n_seg * D * D;
+  const bool carried = p.n_seg > 1 && p.carried;
+  const float* from = carried ? parts + w.seg * D * D : ro.init ? ro.init + bh * D * D : nullptr;
+  if (from) {
+    load_state<D, W>(S, from, carried ? ro.parts_transposed : ro.init_transposed, wave, lane);
+  } else {
+#pragma unroll
+    for (int t = 0; t < D / W; ++t) S[t] = 0.f;
+  }
+  if (carried) return;
+  const int before = ro.reverse ? p.n_seg - 1 - w.seg : w.seg, len = rows_of(p, w.b);
+  for (int i = 0; i < before; ++i) {
+    const int seg = ro.reverse ? p.n_seg - 1 - i : i;
+    typename Layout<W>::Acc sum[D / W];
+    load_state<D, W>(sum, parts + (long)seg * D * D, ro.parts_transposed, wave, lane);
+    const float keep = decay_pow(w.g2, min(max(len - seg * p.seg_rows, 0), p.seg_rows));
+#pragma unroll
+    for (int t = 0; t < D / W; ++t) S[t] = S[t] * keep + sum[t];
+  }
+}
+
 template <class T>
 __device__ __forceinline__ const T* rows_at(const void* base, long ld, int group, const Params& p, const Place& w, int dim) {
   return (const T*)base + ((long)w.b * p.seq + w.s0) * ld + (long)(w.h / group) * dim;
@@ -613,13 +640,7 @@ __global__ __launch_bounds__(256 * H, D == 128 ? 2 : 3) void linattn_walk_kernel
   const long bh = (long)w.b * p.heads + w.h;
 
   Acc S[4];
-  const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
-  if (from) {
-    load_state<D>(S, from, p.n_seg == 1 ? ro.init_transposed : ro.parts_transposed, wave, lane);
-  } else {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) S[t] = 0.f;
-  }
+  entering_state<D>(S, p, ro, w, wave, lane);
   const bool keep_last = p.n_seg == 1 && ro.final_state;
   const uint32_t unit = T::unit(), tr = L::tr(lane), row = L::row(lane);
   const uint32_t unit_xy = L::CROSSED ? T::unit_crossed() : unit, tr_y = L::CROSSED ? L::tr_crossed(lane) : tr;
@@ -905,13 +926,7 @@ __global__ __launch_bounds__(4 * D, 4) void linattn_walk_f32_kernel(Params p) {
   const long bh = (long)w.b * p.heads + w.h;
 
   f32x4 S[DT];
-  const float* from = p.n_seg > 1 ? ro.parts + (bh * p.n_seg + w.seg) * D * D : ro.init ? ro.init + bh * D * D : nullptr;
-  if (from) {
-    load_state<D, 16>(S, from, p.n_seg == 1 ? ro.init_transposed : ro.parts_transposed, wave, lane);
-  } else {
-#pragma unroll
-    for (int t = 0; t < DT; ++t) S[t] = 0.f;
-  }
+  entering_state<D, 16>(S, p, ro, w, wave, lane);
   const bool keep_last = p.n_seg == 1 && ro.final_state;
   const int n = (w.live + kChunkF32 - 1) / kChunkF32;
   const int start = rev ? n - 1 : 0;
@@ -1097,19 +1112,28 @@ __global__ __launch_bounds__(256) void linattn_step_kernel(const E* q, const E* 
 // there with f32 tensors.
 int slots_of(int head_dim, bool f32) { return 256 * (head_dim == 128 ? 2 : f32 ? 4 : 3); }
 
+// Up to how many segments a walk sums those before its own: what it reads then, a state for each, against a launch that carries
+// them.  Heads of 64: forward of 4 x 403 rows of 4 heads, 4 segments, 17.4 us carried and 14.7 summed; 2 x 2220 of 16, 12, 27.3 and
+// 24.6; 1906 of one, 15, 17.9 and 18.6; gradients of 2 x 439 of 16, 4, 21.6 and 17.2; 2 x 1570 of 4, 13, 21.9 and 21.2; 2377 of 2,
+// 19, 19.6 and 21.8.  Heads of 128: forward of 512 rows of 32, 4, 26.6 and 20.0; 2 x 765 of 16, 6, 28.0 and 23.5; 2 x 1128 of one, 9,
+// 22.1 and 24.0; gradients of 2 x 4096 of 32, 5, 215 and 204; 700 of 8, 6, 25.0 and 26.4; 2 x 1225 of one, 10, 23.7 and 34.8.
+int summed_segments(int head_dim, int roles) { return head_dim == 64 ? 12 : roles > 1 ? 5 : 7; }
+
 // Rows of a segment, by an estimate of the time in us: with R rounds of workgroups, each through `rows` rows, and X = 65536ths
 // of all walks' rows
 //   one segment   c0 + c1 R rows + c2 X
-//   n segments    c3 + c4 R rows + c5 X + c6 (n sums' states) / 512 + c7 n
-// (what a workgroup takes through its rows, what all share, the states' way out and in, the chain of the carry).
+//   n segments    c3 + c4 R rows + c5 X + c6 (n sums' states) / 512 + c7 n, the walks summing them; with a carry c8 ..  instead
+// (what a workgroup takes through its rows, what all share, the states' way out and in, the chain through them).
 // Least squares of the relative error over 200 problems of each kind, 1 .. 512 walks of 100 .. 16384 rows in 1 .. 64
-// segments; mean error 5 - 8 %.  Over those the choice costs 0.4 % (bf16) and 2 % (f32) over the best number of segments.  A segment has at
+// segments; mean error 5 - 8 %.  Over those the choice costs 0.8 - 1.5 % over the best number of segments.  A segment has at
 // least 128 rows: below that its state is more to move than they are.
 // One head of 128, 4096 rows: 245 us in one segment, 36 in 32; 3 x 32 heads, 2048 rows: 128 in one, 84 in five.
 constexpr int kSegLeast = 128, kMaxSegments = 64;
-constexpr float kSegFit[2][2][8] = {   // [f32][head 128]
-    {{5.57f, 0.0372f, 2.46f, 10.8f, 0.0484f, 2.68f, 5.28f, 0.372f}, {5.14f, 0.0558f, 4.94f, 12.7f, 0.0774f, 4.52f, 18.7f, 0.35f}},
-    {{4.83f, 0.0701f, 7.07f, 10.5f, 0.1f, 9.25f, 4.48f, 0.367f}, {5.77f, 0.166f, 16.3f, 10.6f, 0.242f, 17.f, 17.7f, 0.344f}}};
+constexpr float kSegFit[2][2][13] = {   // [f32][head 128]
+    {{5.24f, 0.0322f, 2.25f, 6.59f, 0.041f, 2.86f, 2.42f, 0.385f, 10.2f, 0.0401f, 3.29f, 5.11f, 0.14f},
+     {4.94f, 0.0493f, 4.74f, 5.86f, 0.0672f, 4.9f, 6.04f, 1.07f, 10.8f, 0.0644f, 5.49f, 19.3f, 0.14f}},
+    {{4.65f, 0.0688f, 6.59f, 5.4f, 0.0958f, 8.64f, 3.16f, 0.439f, 11.f, 0.0871f, 9.77f, 4.32f, 0.142f},
+     {5.77f, 0.166f, 16.3f, 10.6f, 0.242f, 17.f, 17.7f, 0.344f, 10.6f, 0.242f, 17.f, 17.7f, 0.344f}}};
 
 int segment_rows(const jpp_linattn_args* a, int roles, int sums) {
   const bool f32 = a->dtype == JPP_DTYPE_F32;
@@ -1124,8 +1148,9 @@ int segment_rows(const jpp_linattn_args* a, int roles, int sums) {
     if (rows < kSegLeast) break;
     if (rows >= seq) continue;
     const int64_t segs = (seq + rows - 1) / rows;
-    const float time = f[3] + f[4] * (float)((walks * segs + slots - 1) / slots * rows) + f[5] * x +
-                       f[6] * (float)(heads * sums * segs) / 512.f + f[7] * (float)segs;
+    const float* g = f + (segs <= summed_segments(a->head_dim, roles) ? 3 : 8);
+    const float time = g[0] + g[1] * (float)((walks * segs + slots - 1) / slots * rows) + g[2] * x +
+                       g[3] * (float)(heads * sums * segs) / 512.f + g[4] * (float)segs;
     if (time < least) {
       least = time;
       best = rows;
@@ -1218,7 +1243,6 @@ template <int D, bool F32>
 int launch(hipStream_t st, const Params& p) {
   const int64_t walks = (int64_t)p.batch * p.heads * p.n_roles, sums = (int64_t)p.batch * p.heads * p.n_sums;
   if (p.n_seg > 1) {
-    const unsigned carry = (unsigned)(sums * (D * D / 1024));
     const dim3 grid((unsigned)(sums * p.n_seg));
     if constexpr (F32) {
       hipLaunchKernelGGL((linattn_sum_f32_kernel<D>), grid, dim3(4 * D), 0, st, p);
@@ -1234,8 +1258,10 @@ int launch(hipStream_t st, const Params& p) {
       }
     }
     JPP_LAUNCH_CHECK();
-    hipLaunchKernelGGL((linattn_carry_kernel<D>), dim3(carry), dim3(256), 0, st, p);
-    JPP_LAUNCH_CHECK();
+    if (p.carried) {
+      hipLaunchKernelGGL((linattn_carry_kernel<D>), dim3((unsigned)(sums * (D * D / 1024))), dim3(256), 0, st, p);
+      JPP_LAUNCH_CHECK();
+    }
   }
   if constexpr (F32) {
     hipLaunchKernelGGL((linattn_walk_f32_kernel<D>), dim3((unsigned)(walks * p.n_seg)), dim3(4 * D), 0, st, p);
@@ -1247,7 +1273,9 @@ int launch(hipStream_t st, const Params& p) {
   JPP_LAUNCH_CHECK();
   return JPP_OK;
 }
-int launch_any(hipStream_t st, const Params& p, const jpp_linattn_args* a) {
+int launch_any(hipStream_t st, Params p, const jpp_linattn_args* a) {
+  p.carried = p.n_seg > summed_segments(a->head_dim, p.n_roles);
+  for (int i = 0; i < p.n_sums; ++i) p.carried |= p.role[i].final_state != nullptr;   // (which may lie over what enters)
   const bool f32 = a->dtype == JPP_DTYPE_F32;
   if (a->head_dim == 64) return f32 ? launch<64, true>(st, p) : launch<64, false>(st, p);
   return f32 ? launch<128, true>(st, p) : launch<128, false>(st, p);

@@ -363,3 +363,39 @@ def test_rows_far_apart(f32, dim):
     size = (O.linattn(*sizes[:3], *args)[0], *O.linattn_bwd(*sizes, *args)[:3])
     for i, name in enumerate(names[4:]):
         _close(got[None, :, None, 4 + i], want[i], size[i], f32, name)
+
+
+@pytest.mark.parametrize("batch,seq,heads,kv,lens", [(1, 500, 32, 16, None), (1, 900, 24, 4, [700]), (2, 450, 20, 5, [450, 129])])
+def test_heads_in_pairs_and_segments(batch, seq, heads, kv, lens):
+    """The same where sequences are cut into a few segments, whose walks sum those before their own."""
+    Problem(batch, seq, heads, kv, 128, lens=lens, states=False, seed=11).check_backward()
+    p = Problem(batch, seq, heads, kv, 128, lens=lens, seed=12)
+    p.check_backward()
+    p.check_forward()
+
+
+@pytest.mark.parametrize("f32", [False, True], ids=["bf16", "f32"])
+@pytest.mark.parametrize("dim,seq", [(64, 400), (64, 1500), (64, 2300), (128, 400), (128, 600), (128, 1500)])
+def test_states_that_enter_segments(dim, seq, f32):
+    """A state that enters and none that is asked for: summed by the walks, or carried, by the number of segments."""
+    p = Problem(2, seq, 2, 2, dim, f32, lens=[seq, seq - 171], seed=13)
+    s = p.sizes
+    args, sizes = (p.decay, s["scale"]), [np.abs(a) for a in (p.q, p.k, p.v, p.d_o)]
+    dev, dev_back = p._common(False), p._common(True)
+    o, dq, dk, dv = (Tensor(np.full(a.shape, 7.0), f32, p.pad) for a in (p.q, p.q, p.k, p.v))
+    state, d_state = _up(p.state), _up(p.d_state)
+    rt.linattn_fwd(dev["q"].ptr, dev["k"].ptr, dev["v"].ptr, o.ptr, dev["decay"].ptr, dev["q"].ld, dev["k"].ld, dev["v"].ld, o.ld,
+                   state_in=state.ptr, lens=dev["lens"].ptr, workspace=dev["workspace"].ptr, **s)
+    d = dev_back
+    rt.linattn_bwd(d["q"].ptr, d["k"].ptr, d["v"].ptr, d["d_o"].ptr, dq.ptr, dk.ptr, dv.ptr, d["decay"].ptr, d["q"].ld, d["k"].ld,
+                   d["v"].ld, d["d_o"].ld, dq.ld, dk.ld, dv.ld, state_in=state.ptr, d_state_out=d_state.ptr, lens=d["lens"].ptr,
+                   workspace=d["workspace"].ptr, **s)
+    rt.sync()
+    p._guard(dev)
+    p._guard(dev_back)
+    _close(o.get(), O.linattn(p.q, p.k, p.v, *args, p.state, p.lens)[0],
+           O.linattn(*sizes[:3], *args, np.abs(p.state), p.lens)[0], f32, "o")
+    want = O.linattn_bwd(p.q, p.k, p.v, p.d_o, *args, p.state, p.d_state, p.lens)
+    size = O.linattn_bwd(*sizes, *args, np.abs(p.state), np.abs(p.d_state), p.lens)
+    for name, got, w, m in zip(("dq", "dk", "dv"), (dq, dk, dv), want, size):
+        _close(got.get(), w, m, f32, name)
