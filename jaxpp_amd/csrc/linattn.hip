@@ -605,7 +605,7 @@ __global__ __launch_bounds__(256) void linattn_carry_kernel(Params p) {
 // The state is held over a factor m that takes the decays, so that most chunks leave the accumulators alone: m falls by
 // lambda^rows a chunk, the new terms are divided by it, and below 2^-20 it is multiplied in.
 // PARTS: of the state's terms, see update_state.
-// 16384 rows of 32 heads of 128, forward: 122 us, 4.4 TB/s; gradients of 2 x 4096 rows of 32 heads on 8: 175 us, there the phases of
+// 16384 rows of 32 heads of 128, forward: 118 us, 4.6 TB/s; gradients of 2 x 4096 rows of 32 heads on 8: 198 us, there the phases of
 // a chunk one after the other at two waves a SIMD (matrix cores 32 % of the time, vector instructions 30 %, LDS 27 %; no phase alone
 // is worth more than 42 us).
 // Three workgroups of heads of 64 fit a CU's LDS; registers for a fourth would be spilled ones (gradients of 2 x 4096 x 32
